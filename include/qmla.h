@@ -309,6 +309,103 @@ typedef struct qmla_prep_params {
 
 int qmla_prep(const qmla_prep_params* p, void* stream);
 
+/* ---- rotary positions -------------------------------------------------------------------------
+ * Rotates `rot` columns [offset, offset + rot) of every query and key head by the angles of its token's
+ * position: pair i of a head, (x, y), becomes (x cos_i - y sin_i, y cos_i + x sin_i), and with `inverse`
+ * the rotation back. Pairs are columns (i, i + rot/2) in the half layout, (2i, 2i + 1) in the interleaved
+ * one. cos_sin holds fp32 rows [cos_0 .. cos_{rot/2-1} | sin_0 ..] per position, so a context scaling is
+ * the table's. fp32 arithmetic, rounded once to the heads' type. The other columns are copied, or left
+ * alone where an output is its input (q_out == q with equal strides). A position outside [0, max_pos)
+ * gives NaN in the rotated columns. The reference rotates inside its attention module only, in bf16
+ * arithmetic (qwen_mla/qwen3_5_mla.py:341-354, qmla_prep here). Asynchronous, allocates nothing. */
+typedef struct qmla_rotary_params {
+  const void* q;                  /* [n, q_heads, head_dim]; strides in elements */
+  int64_t q_token_stride, q_head_stride;
+  const void* k;                  /* [n, k_heads, head_dim], k_heads 0: none */
+  int64_t k_token_stride, k_head_stride;
+  void* q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  void* k_out;
+  int64_t k_out_token_stride, k_out_head_stride;
+  const int64_t* positions;       /* [n], elements pos_stride apart */
+  int64_t pos_stride;
+  const float* cos_sin;           /* [max_pos, rot] */
+  int64_t max_pos, cos_sin_stride;
+  int32_t n, q_heads, k_heads, head_dim, offset, rot;
+  int32_t interleaved, inverse;
+  int32_t dtype;                  /* QMLA_DT_* of q, k and their outputs */
+} qmla_rotary_params;
+
+int qmla_rotary(const qmla_rotary_params* p, void* stream);
+
+/* ---- eviction: which tokens a request keeps, and their rows moved together -------------------------
+ * qmla_evict_select: request b of length L = min(seq_lens[b], width) keeps all its tokens if L <= keep,
+ * else `keep` of them: the first `sink`, the last `recent`, and of the others the heaviest by weights[b, t],
+ * ties to the lower token; a NaN weight counts as -inf. index[b, 0 .. counts[b]) are the kept tokens in
+ * ascending order, the rest of the row (up to keep) is -1. sink + recent <= keep.
+ * qmla_cache_compact: the cached row of token index[b, i] of request b (pages block_table[b]) is copied
+ * to token first[b] + i (0 + i without `first`) of request b's destination pages, for i < counts[b],
+ * and, when weights_out is given, weights_out[b, first[b] + i] = weights[b, index[b, i]].
+ * dst_block_table NULL: in place, into the request's own pages; index[b] must then ascend strictly with
+ * index[b, i] >= first[b] + i, and no other request may share the pages. Else the destination pages must
+ * be none of the source pages. Rows that name a page or token outside the tables are not copied and
+ * store QMLA_ERR_PAGE into *status. Neither has a counterpart in the reference. Both asynchronous,
+ * neither allocates. */
+typedef struct qmla_evict_params {
+  const float* weights;           /* [requests, width], row stride weights_stride; NULL in a compact
+                                     that moves none */
+  int64_t weights_stride;
+  const int32_t* seq_lens;        /* select: [requests] */
+  int32_t* index;                 /* [requests, keep], row stride index_stride (select writes it) */
+  int64_t index_stride;
+  int32_t* counts;                /* [requests] (select writes it) */
+  int32_t requests, width, keep, sink, recent;
+  /* compact */
+  void* cache;                    /* [num_pages, page_size, (1,) row] */
+  int64_t page_stride, token_stride;   /* bytes */
+  int64_t row_bytes;              /* bytes copied per row */
+  int32_t page_size, num_pages;
+  const int32_t* block_table;     /* [requests, bt_cols] */
+  int64_t bt_stride;
+  int32_t bt_cols;
+  const int32_t* dst_block_table; /* [requests, dst_bt_cols], NULL: in place */
+  int64_t dst_bt_stride;
+  int32_t dst_bt_cols;
+  const int32_t* first;           /* [requests] or NULL */
+  float* weights_out;             /* [requests, weights_out_width] or NULL; may be `weights` in place */
+  int64_t weights_out_stride;
+  int32_t weights_out_width;
+  int32_t* status;
+} qmla_evict_params;
+
+int qmla_evict_select(const qmla_evict_params* p, void* stream);
+int qmla_cache_compact(const qmla_evict_params* p, void* stream);
+
+/* ---- attention weight of every cached token -------------------------------------------------------
+ * out[b, t] = (weights ? weights[b, t] : 0) + sum over the request's qrows query rows and heads of
+ * exp(s - lse[row, head]) for t < L_b, s the score qmla_decode forms from the same params (queries,
+ * cache, divisors, sm_scale, logit_cap; row j of a request sees its first L_b - (qrows-1-j) tokens) and
+ * lse what it returned (fp32, rows with lse -inf add nothing). Columns from L_b on are left as they
+ * were; L_b is cut to `width`. out may be `weights`. p->out, p->lse, the split and workspace fields are
+ * ignored. The sum's order is fixed: the same inputs give the same bits. No counterpart in the
+ * reference. Asynchronous, allocates nothing. */
+int qmla_attention_weights(const qmla_decode_params* p, const float* lse, int64_t lse_stride, const float* weights,
+                           int64_t weights_stride, float* out, int64_t out_stride, int32_t width, void* stream);
+
+/* ---- attention of a tree of drafted tokens ---------------------------------------------------------
+ * One request drafts up to qrows = p->qrows <= 64 tokens that form a tree, its rows at the end of the
+ * request's cached tokens: node i of a request with n nodes (node_counts[b], or qrows without them) is
+ * token L_b - n + i. Query row j < n (node j) sees the L_b - n tokens before the nodes and the nodes i
+ * with bit i of tree_mask[b, j] set; rows from n on see nothing. p is qmla_decode's block with rows =
+ * requests * qrows, except that block_table and seq_lens hold ONE row per request and that the split
+ * fields are ignored; groups must be 1. Rows that see no token get a zero output and lse -inf. A
+ * non-finite element in a drafted token's cached row makes the rows that see it NaN, others not.
+ * `workspace` of qmla_tree_workspace_bytes() holds partial results. The reference verifies chains only
+ * (qwen_mla/mla_impl.py:628-662). Asynchronous, allocates nothing. */
+size_t qmla_tree_workspace_bytes(const qmla_decode_params* p);
+int qmla_tree_forward(const qmla_decode_params* p, const int64_t* tree_mask, int64_t mask_stride,
+                      const int32_t* node_counts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,10 @@ SOURCES = [
     (CSRC / "qmla_wsb.hip", ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"]),
     (CSRC / "qmla_write.hip", []),
     (CSRC / "qmla_prep.hip", []),
+    (CSRC / "qmla_rotary.hip", []),
+    (CSRC / "qmla_evict.hip", []),
+    (CSRC / "qmla_weights.hip", ["-mllvm", "-amdgpu-mfma-vgpr-form"]),
+    (CSRC / "qmla_tree.hip", []),
 ]
 
 

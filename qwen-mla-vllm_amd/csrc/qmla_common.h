@@ -426,6 +426,14 @@ inline bool rows16(const qmla_decode_params* p) {
   return ((uintptr_t)p->kv_cache & 15) == 0 && (p->page_stride * eb) % 16 == 0 && (p->token_stride * eb) % 16 == 0;
 }
 
+// ---- host-side interface of the main translation unit (qmla_decode.hip) ----
+// Compute units of the current device.
+int cu_count();
+// The checks of a decode parameter block for kernels that read no column past d_c + rope_w.
+int validate_params(const qmla_decode_params* p);
+// A checked parameter block as the kernels take it (num_splits > 0: no plan, no balanced partials).
+KParams make_kparams(const qmla_decode_params* p);
+
 // ---- host-side interface of the warp-specialized translation unit (qmla_ws.hip) ----
 int ws_select(const qmla_decode_params* p);
 int ws_head_split(const qmla_decode_params* p);

@@ -989,7 +989,7 @@ static const Inst kInst[] = {
 
 static int g_cu_count[64];
 
-static int cu_count() {
+int cu_count() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
   if (g_cu_count[dev] == 0) {
@@ -1017,9 +1017,9 @@ static int wp_of(int rope_w) { return (rope_w + 63) / 64 * 64; }
 
 // staged bytes per row: scores read [0, (d_c + WP)*EB) (the padded pair is masked but still read),
 // plus the rms tail
-static int64_t needed_row_bytes(const qmla_decode_params* p) {
+static int64_t needed_row_bytes(const qmla_decode_params* p, bool pad = true) {
   const int eb = elem_bytes(p->kv_dtype);
-  int64_t need = (int64_t)(p->d_c + wp_of(p->rope_w)) * eb;
+  int64_t need = (int64_t)(p->d_c + (pad ? wp_of(p->rope_w) : p->rope_w)) * eb;
   if (p->rms_mode != QMLA_RMS_NONE) {
     const int64_t rms_end = (int64_t)p->rms_offset * eb + (int64_t)p->rms_heads * rms_elem_bytes(p);
     if (rms_end > need) need = rms_end;
@@ -1030,8 +1030,9 @@ static int64_t needed_row_bytes(const qmla_decode_params* p) {
 static bool aligned16(const void* ptr) { return ((uintptr_t)ptr & 15) == 0; }
 
 // Checks of a parameter block; `ptrs` = false checks the shapes and modes only (no pointers, no
-// address alignment), for questions asked before the tensors exist.
-static int validate(const qmla_decode_params* p, bool ptrs = true) {
+// address alignment), for questions asked before the tensors exist. `pad`: the kernel stages the rope
+// columns in 64-column steps, so a row must hold them.
+static int validate(const qmla_decode_params* p, bool ptrs = true, bool pad = true) {
   if (!p) return QMLA_ERR_NULL;
   if (ptrs && (!p->q_nope || !p->kv_cache || !p->block_table || !p->seq_lens || !p->out)) return QMLA_ERR_NULL;
   if (ptrs && p->rope_w > 0 && !p->q_pe) return QMLA_ERR_NULL;
@@ -1058,7 +1059,7 @@ static int validate(const qmla_decode_params* p, bool ptrs = true) {
   // 4-byte boundaries here; rows off 16-byte boundaries are served by the narrow-row instances only
   if ((ptrs && (uintptr_t)p->kv_cache % 4) || (p->page_stride * eb) % 4 || (p->token_stride * eb) % 4)
     return QMLA_ERR_ALIGN;
-  if (needed_row_bytes(p) > p->token_stride * eb && p->page_size > 1) return QMLA_ERR_SHAPE;
+  if (needed_row_bytes(p, pad) > p->token_stride * eb && p->page_size > 1) return QMLA_ERR_SHAPE;
   // queries: element alignment (16-byte aligned rows take the vector loads)
   if (ptrs && ((uintptr_t)p->q_nope % 2 || (p->rope_w > 0 && (uintptr_t)p->q_pe % 2))) return QMLA_ERR_ALIGN;
   return QMLA_OK;
@@ -1155,7 +1156,9 @@ static int plan_switch(const qmla_decode_params* p) {
   return kPlanSwitchOther;
 }
 
-static KParams make_kparams(const qmla_decode_params* p) {
+int validate_params(const qmla_decode_params* p) { return validate(p, true, false); }
+
+KParams make_kparams(const qmla_decode_params* p) {
   KParams k;
   const int eb = elem_bytes(p->kv_dtype);
   k.q_vec = aligned16(p->q_nope) && (p->q_nope_stride_row * 2) % 16 == 0 && (p->q_nope_stride_head * 2) % 16 == 0 &&

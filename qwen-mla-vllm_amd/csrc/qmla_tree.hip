@@ -1,0 +1,622 @@
+// Attention of a tree of drafted tokens over the paged latent cache (qmla_tree_forward). See
+// include/qmla.h for what a node sees.
+//
+// A request's nodes x heads are its query rows (node-major, so a row's head is row % heads), up to
+// 64 x heads of them on one latent: a matrix-core problem, not a streaming one like the decode. A
+// workgroup of four waves holds ROWS of them and walks the request's tokens in tiles of 32:
+//   S^T = K Q^T   v_mfma_f32_32x32x16_bf16, keys from LDS as A, queries in registers as B, so a lane
+//                 holds one row's scores of 16 tokens and the softmax needs one exchange with the lane
+//                 32 away;
+//   O^T = V^T P^T the same product, values by transposed LDS reads as A; P stays in the registers the
+//                 scores came in (their token order 8(i/4) + 4(lane/32) + i%4 is the order the two
+//                 transposed reads of a fragment fetch).
+// With NS = 1 a wave owns 32 rows whole. Wider latents do not fit one wave's registers (32 rows x d_c fp32
+// and 32 rows of queries): NS waves share 32 rows, each with 1/NS of the score columns and of the output
+// columns, and add their partial scores through LDS in one order, so they hold equal scores.
+// FP8 rows become bf16 on their way into LDS (exact). P is bf16, the sum that normalizes is of the same
+// rounded P, the lse of the unrounded.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qmla.h"
+#include "qmla_common.h"
+
+namespace qmla {
+namespace tr {
+
+constexpr int TT = 32, NT = 256;
+constexpr int LDS_MAX = 160 * 1024;
+constexpr int MAXH = 64;
+constexpr float kMoveAt = 8.f;   // log2 units a row's maximum may pass its softmax reference by
+
+struct TrParams {
+  KParams k;
+  const int64_t* mask;
+  int64_t mask_sr;
+  const int* counts;
+  int rt;              // row tiles of a request
+  int rows;            // query rows of a request
+  int cols;            // d_c + rope_w
+  int nwg, min_chunk;
+  int rms_mode, rms_b;
+  int64_t* plan;       // [0] chunk, [1 + b] tiles before request b
+  float* part_o;
+  float* part_lse;
+};
+
+__device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int node_count(const TrParams& t, int b) {
+  const int n = t.counts ? t.counts[b] : t.k.qrows;
+  return n < 0 ? 0 : n < t.k.qrows ? n : t.k.qrows;
+}
+__device__ __forceinline__ int tiles_of(const TrParams& t, int b) {
+  const int L = t.k.seq_lens[b];
+  return L <= 0 || node_count(t, b) == 0 ? 0 : (L + TT - 1) / TT;
+}
+
+// Work units are (row tile, token tile) pairs, requests outermost, tokens innermost; workgroup w owns units
+// [w * chunk, (w + 1) * chunk).
+struct Range {
+  int64_t lo, hi, chunk;
+  int b;
+  int64_t c0;   // units before request b
+};
+__device__ inline Range unit_range(const TrParams& t, int w, bool store) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int base = 0; base < t.k.n_req; base += 64) {
+    const int b = base + lane;
+    total += lane_value(wave_incl_sum(b < t.k.n_req ? tiles_of(t, b) : 0), 63);
+  }
+  Range r;
+  const int64_t units = total * t.rt;
+  r.chunk = (units + t.nwg - 1) / t.nwg;
+  if (r.chunk < t.min_chunk) r.chunk = t.min_chunk;
+  r.lo = w * r.chunk;
+  r.hi = r.lo + r.chunk < units ? r.lo + r.chunk : units;
+  r.b = 0;
+  r.c0 = 0;
+  if (store && lane == 0) t.plan[0] = r.chunk;
+  if (r.lo >= r.hi && !store) return r;
+  int64_t run = 0;
+  for (int base = 0; base < t.k.n_req; base += 64) {
+    const int b = base + lane;
+    const int n = b < t.k.n_req ? tiles_of(t, b) : 0;
+    const int in = wave_incl_sum(n);
+    const int64_t c = run + in - n;
+    if (store && b < t.k.n_req) t.plan[1 + b] = c;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(b < t.k.n_req && c * t.rt <= r.lo);
+    if (m) {
+      const int x = 63 - __builtin_clzll(m);
+      r.b = base + x;
+      r.c0 = (run + lane_value(in - n, x)) * t.rt;
+    }
+    run += lane_value(in, 63);
+  }
+  return r;
+}
+
+// Staged tile: 32 rows of CP bf16 columns in 16-byte chunks, chunk c of row r at c ^ swz(r) inside its
+// aligned group. Over 32 chunks of 16 bytes (128 banks) a row's stride takes `b` of the row's five bits apart;
+// the others are spread by the swizzle, low ones first onto the 4-chunk bit: 32 rows' same chunk (score
+// reads) and 8 rows' same 4 chunks (value reads) then lie on distinct banks.
+template <int RS>
+__device__ __forceinline__ int swz(int r) {
+  static_assert(RS % 8 == 0);
+  constexpr int b = RS % 32 == 0 ? 0 : RS % 32 == 16 ? 1 : 2, n = 5 - b;
+  const int x = (r & 31) >> b;
+  return ((x & ((1 << (n - 2)) - 1)) << 2) | (x >> (n - 2));
+}
+
+__device__ __forceinline__ float inv_divisor(uint32_t raw, int mode, float ks) {
+  if (mode == QMLA_RMS_LOG8) return fast_exp2(3.0f - (float)raw * (6.0f / 255.0f));
+  if (mode == QMLA_RMS_NONE) return 1.f;
+  const float r = mode == QMLA_RMS_E4M3 ? fp8_to_f32(raw) * ks : bf16_bits_to_f32(raw);
+  return r > 0.f ? 1.f / r : 1.f;
+}
+
+// any element of 16 bytes not finite
+template <bool FP8>
+__device__ __forceinline__ bool any_odd(const i32x4& v) {
+  bool odd = false;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t u = (uint32_t)v[d];
+    if constexpr (FP8) {
+      const uint32_t x = (u & 0x7f7f7f7fu) + 0x01010101u;   // 0x7f becomes 0x80
+      odd = odd || (x & 0x80808080u);
+    } else {
+      odd = odd || (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  return odd;
+}
+
+template <bool FP8_, int DC_, int CP_, int NS_, int STAGES_>
+struct Cfg {
+  static constexpr bool FP8 = FP8_;
+  static constexpr int DC = DC_, CP = CP_, NS = NS_, STAGES = STAGES_;
+  static constexpr int ROWS = 128 / NS;            // query rows of a workgroup
+  static constexpr int RS = CP / 8;                // 16-byte chunks of a staged row
+  static constexpr int QC = CP / NS, NQ = QC / 16; // score columns of a wave, its products
+  static constexpr int OB = DC / NS / 32;          // output column blocks of a wave
+  static constexpr int UC = FP8 ? 16 : 8;          // columns of a 16-byte load
+  static constexpr int UPR = CP / UC;              // loads of a row
+  static constexpr int LOADS = (TT * UPR + NT - 1) / NT;
+  static constexpr int TILE_B = TT * CP * 2;
+  static_assert(DC % (32 * NS) == 0 && CP % (16 * NS) == 0 && CP % 64 == 0);
+};
+
+constexpr int IRS = TT + 4;   // floats of a head's divisors in LDS
+
+template <class C>
+__host__ __device__ constexpr int lds_bytes(int heads) {
+  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 2 * TT * 8 + 16;
+}
+
+template <class C>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_kernel(const TrParams t) {
+  extern __shared__ __align__(16) char lds[];
+  const KParams& p = t.k;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int rg = wave / C::NS, cp = wave % C::NS;
+  char* kt = lds;
+  float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [STAGES][heads][IRS]
+  char* part = lds + C::STAGES * (C::TILE_B + p.heads * IRS * 4);        // [4 waves][4][64] 16 bytes
+  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [2][TT]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(rowoff + 2 * TT);          // [3], bit per token
+  // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
+  const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const Range rng = unit_range(t, w, w == 0);
+  if (rng.lo >= rng.hi) return;
+  const float ks = p.k_scale ? *p.k_scale : 1.f;
+  const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
+  int bad = 0;
+  int64_t u = rng.lo, c0 = rng.c0;
+  int b = rng.b;
+  while (u < rng.hi) {
+    const int nt = tiles_of(t, b);
+    if (u >= c0 + (int64_t)nt * t.rt) {
+      c0 += (int64_t)nt * t.rt;
+      ++b;
+      continue;
+    }
+    const int m = (int)((u - c0) / nt), ta = (int)((u - c0) - (int64_t)m * nt);
+    const int te = rng.hi - u < nt - ta ? ta + (int)(rng.hi - u) : nt;
+    const int L = p.seq_lens[b], nodes = node_count(t, b), base = L - nodes;
+    // ---- this lane's query row
+    const int r0 = m * C::ROWS + rg * 32, r = r0 + n;
+    const bool wlive = r0 < t.rows;
+    const bool rvalid = r < t.rows;
+    const int node = rvalid ? r / p.heads : 0, head = rvalid ? r - node * p.heads : 0;
+    const bool rlive = rvalid && node < nodes;
+    const uint64_t sees = rlive ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
+    bf16x8 qf[C::NQ];
+    {
+      const int64_t row = (int64_t)b * p.qrows + node;
+      const __bf16* qn = p.q_nope + row * p.qn_sr + head * p.qn_sh;
+      const __bf16* qp = p.q_pe + row * p.qp_sr + head * p.qp_sh;
+#pragma unroll
+      for (int f = 0; f < C::NQ; ++f) {
+        const int c = cp * C::QC + 16 * f + 8 * h;
+        bf16x8 v{};
+        if (rlive) {
+          if (c < C::DC) {
+            v = load_q8(qn + c, p.q_vec);
+          } else if (c - C::DC + 8 <= p.rope_w) {
+            v = load_q8(qp + (c - C::DC), p.q_vec);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c - C::DC + i < p.rope_w) v[i] = qp[c - C::DC + i];
+          }
+        }
+        qf[f] = v;
+      }
+    }
+    f32x16 acc[C::OB];
+#pragma unroll
+    for (int i = 0; i < C::OB; ++i) acc[i] = f32x16{};
+    float m_ref = kNegInf, l_sum = 0.f, l_p = 0.f;
+
+    // ---- staging
+    i32x4 raw[C::LOADS];
+    constexpr int RL = MAXH * TT / NT;
+    uint32_t rraw[RL];
+    auto rows_of = [&](int j) {   // byte offsets of tile j's rows
+      if (tid < TT) {
+        const int tok = j * TT + tid;
+        int64_t off = -1;
+        if (tok < L) {
+          const int pg = page_div(p, tok);
+          const int id = checked_page(p, p.bt[b * p.bt_stride + pg], bad);
+          off = id * p.page_stride_b + (int64_t)(tok - pg * p.page_size) * p.token_stride_b;
+        }
+        rowoff[(j & 1) * TT + tid] = off;
+      }
+    };
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i) {
+        const int q = i * NT + tid, row = q / C::UPR, c = q % C::UPR;
+        raw[i] = i32x4{};
+        if (q < TT * C::UPR) {
+          const int64_t off = rowoff[(j & 1) * TT + row];
+          if (off >= 0 && c * C::UC < t.cols) raw[i] = *reinterpret_cast<const i32x4*>(p.kv + off + 16 * c);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RL; ++i) {
+        const int q = i * NT + tid;
+        rraw[i] = 0;
+        if ((q >> 5) < p.heads && t.rms_mode != QMLA_RMS_NONE) {
+          const int64_t off = rowoff[(j & 1) * TT + (q & 31)];
+          if (off >= 0) {
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(p.kv + off + p.rms_off_b + (q >> 5) * t.rms_b);
+            rraw[i] = t.rms_b == 2 ? at[0] | ((uint32_t)at[1] << 8) : at[0];
+          }
+        }
+      }
+    };
+    auto put = [&](int j) {
+      char* dst = kt + (C::STAGES > 1 ? (j & 1) * C::TILE_B : 0);
+      const bool drafted = (j + 1) * TT > base;
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i) {
+        const int q = i * NT + tid, row = q / C::UPR, c = q % C::UPR;
+        if (q < TT * C::UPR) {
+          i32x4 v = raw[i];
+          const int left = t.cols - c * C::UC;
+          if (left < C::UC) {   // the divisors begin inside this load
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const int bits = left * (C::FP8 ? 8 : 16) - 32 * d;
+              v[d] = bits <= 0 ? 0 : bits >= 32 ? v[d] : v[d] & (int)((1u << bits) - 1);
+            }
+          }
+          if (drafted && j * TT + row >= base && any_odd<C::FP8>(v)) {
+            atomicOr(&odd[j % 3], 1u << row);
+            v = i32x4{};
+          }
+          const int s = swz<C::RS>(row);
+          char* at = dst + row * (C::CP * 2);
+          if constexpr (C::FP8) {
+            bf16x8 x, y;
+            fp8x16_to_bf16(v, x, y);
+            *reinterpret_cast<bf16x8*>(at + (((2 * c) ^ s) << 4)) = x;
+            *reinterpret_cast<bf16x8*>(at + (((2 * c + 1) ^ s) << 4)) = y;
+          } else {
+            *reinterpret_cast<i32x4*>(at + ((c ^ s) << 4)) = v;
+          }
+        }
+      }
+      float* ir = irms + (C::STAGES > 1 ? (j & 1) * p.heads * IRS : 0);
+#pragma unroll
+      for (int i = 0; i < RL; ++i) {
+        const int q = i * NT + tid;
+        if ((q >> 5) < p.heads) ir[(q >> 5) * IRS + (q & 31)] = fs * inv_divisor(rraw[i], t.rms_mode, ks);
+      }
+    };
+
+    __syncthreads();   // the last piece's tiles are read
+    if (tid < 3) odd[tid] = 0;
+    rows_of(ta);
+    __syncthreads();
+    fetch(ta);
+    if (ta + 1 < te) rows_of(ta + 1);
+    put(ta);
+    __syncthreads();
+
+    for (int j = ta; j < te; ++j) {
+      const char* src = kt + (C::STAGES > 1 ? (j & 1) * C::TILE_B : 0);
+      if (j + 1 < te) fetch(j + 1);
+      if (j + 2 < te) rows_of(j + 2);
+      if (tid == 0) odd[(j + 2) % 3] = 0;
+      // ---- scores
+      f32x16 s{};
+      if (wlive) {
+        const char* krow = src + n * (C::CP * 2);
+        const int sw = swz<C::RS>(n);
+#pragma unroll
+        for (int f = 0; f < C::NQ; ++f) {
+          const int c = cp * (C::QC / 8) + 2 * f + h;
+          s = mfma32(*reinterpret_cast<const bf16x8*>(krow + ((c ^ sw) << 4)), qf[f], s);
+        }
+      }
+      if constexpr (C::NS > 1) {
+        if (wlive) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            *reinterpret_cast<f32x4*>(part + ((wave * 4 + i4) * 64 + lane) * 16) =
+                f32x4{s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]};
+        }
+        __syncthreads();
+        if (wlive) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            f32x4 sum = *reinterpret_cast<const f32x4*>(part + ((rg * C::NS * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int x = 1; x < C::NS; ++x) sum += *reinterpret_cast<const f32x4*>(part + (((rg * C::NS + x) * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * i4 + i] = sum[i];
+          }
+        }
+      }
+      if (wlive) {
+        // ---- divide, cap, mask
+        const float* ir = irms + (C::STAGES > 1 ? (j & 1) * p.heads * IRS : 0) + head * IRS + 4 * h;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
+        }
+        if (p.logit_cap > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[i] = p.logit_cap * kLog2e * (1.0f - 2.0f / (fast_exp2(2.0f * kLog2e * (s[i] / p.logit_cap)) + 1.0f));
+        }
+        if ((j + 1) * TT > base) {
+          const uint32_t od = odd[j % 3];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
+            const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
+            s[i] = !vis ? kNegInf : (od >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
+          }
+        }
+        // ---- softmax against a reference that moves when a row's maximum has passed it by kMoveAt
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        {
+          const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+        }
+        // (a row's own doing: what its neighbours hold does not move it; a NaN maximum moves nothing)
+        const bool moves = mx > m_ref + kMoveAt;
+        if (__builtin_amdgcn_ballot_w64(moves)) {
+          const float alpha = moves ? fast_exp2(m_ref - mx) : 1.f;
+          l_sum *= alpha;
+          l_p *= alpha;
+#pragma unroll
+          for (int ob = 0; ob < C::OB; ++ob) acc[ob] *= alpha;
+          m_ref = moves ? mx : m_ref;
+        }
+        const float m_use = is_neg_inf(m_ref) ? 0.f : m_ref;
+        bf16x8 pf[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = fast_exp2(s[i] - m_use);
+          l_sum += e;
+          const __bf16 e16 = (__bf16)e;
+          l_p += (float)e16;
+          pf[i >> 3][i & 7] = e16;
+        }
+        // ---- values
+        {
+          const int q = lane & 15, rr = 4 * h + (q >> 2);
+#pragma unroll
+          for (int ob = 0; ob < C::OB; ++ob) {
+            const int col = cp * (C::DC / C::NS) + 32 * ob + 16 * ((lane >> 4) & 1) + 4 * (q & 3);
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+              i16x4 v[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int row = 16 * k2 + 8 * x + rr;
+                const char* at = src + row * (C::CP * 2) + (((col >> 3) ^ swz<C::RS>(row)) << 4) + (col & 4) * 2;
+                v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(QMLA_LDS(i16x4, at));
+              }
+              typedef short i16x8 __attribute__((ext_vector_type(8)));
+              const i16x8 va = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+              acc[ob] = mfma32(__builtin_bit_cast(bf16x8, va), pf[k2], acc[ob]);
+            }
+          }
+        }
+      }
+      if constexpr (C::STAGES == 1) __syncthreads();
+      if (j + 1 < te) put(j + 1);
+      __syncthreads();
+    }
+
+    // ---- this piece's rows
+    if (wlive && rvalid) {
+      {
+        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_sum), __float_as_uint(l_sum), false, false);
+        l_sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+        const auto o2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_p), __float_as_uint(l_p), false, false);
+        l_p = __uint_as_float(o2[0]) + __uint_as_float(o2[1]);
+      }
+      if (!rlive) l_sum = l_p = 0.f;
+      const bool whole = ta == 0 && te == nt;
+      const int64_t slot = 2 * w + (u > rng.lo ? 1 : 0);
+      const float inv = empty_sum(l_p) ? 0.f : (whole ? ks : 1.f) / l_p;
+      const int col = cp * (C::DC / C::NS) + 4 * h;
+      const int64_t orow = whole ? ((int64_t)b * p.qrows + node) * p.o_sr + head * p.o_sh : (slot * C::ROWS + rg * 32 + n) * C::DC;
+      const int dt = whole ? p.out_dt : QMLA_DT_F32;
+      char* ob0 = (whole ? reinterpret_cast<char*>(p.out) : reinterpret_cast<char*>(t.part_o)) + (orow + col) * out_bytes(dt);
+      auto store = [&](auto dtc) {
+        constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
+#pragma unroll
+        for (int ob = 0; ob < C::OB; ++ob)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
+            store_out4<DT>(ob0 + (32 * ob + 8 * i4) * ES, v);
+          }
+      };
+      if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
+      else if (dt == QMLA_DT_F16) store(std::integral_constant<int, QMLA_DT_F16>{});
+      else store(std::integral_constant<int, QMLA_DT_BF16>{});
+      if (h == 0 && cp == 0) {
+        if (!whole) t.part_lse[slot * C::ROWS + rg * 32 + n] = empty_sum(l_sum) ? kNegInf : m_ref + fast_log2(l_sum);
+        else if (p.lse) store_out(p.lse, p.lse_dt, ((int64_t)b * p.qrows + node) * p.lse_sr + head, row_lse(m_ref, l_sum));
+      }
+    }
+    u += te - ta;
+  }
+  report_pages(p, bad);
+}
+
+// Rows whose tokens several workgroups shared, and rows of requests without tokens. A wave a row.
+template <int DC, int ROWS>
+__global__ __launch_bounds__(256) void tree_combine_kernel(const TrParams t) {
+  const KParams& p = t.k;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = blockIdx.x * 4 + wave, m = blockIdx.y, b = blockIdx.z, r = m * ROWS + x;
+  if (r >= t.rows) return;
+  const int node = r / p.heads, head = r - node * p.heads;
+  const int64_t row = (int64_t)b * p.qrows + node;
+  const int64_t o = row * p.o_sr + head * p.o_sh;
+  const int nt = tiles_of(t, b);
+  if (nt == 0) {
+    for (int c = lane; c < DC; c += 64) store_out(p.out, p.out_dt, o + c, 0.f);
+    if (lane == 0 && p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, kNegInf);
+    return;
+  }
+  const int64_t chunk = t.plan[0], u0 = t.plan[1 + b] * t.rt + (int64_t)m * nt, u1 = u0 + nt;
+  const int w0 = (int)(u0 / chunk), w1 = (int)((u1 - 1) / chunk);
+  if (w0 == w1) return;
+  auto at = [&](int w) {
+    const int64_t start = u0 > w * chunk ? u0 : w * chunk;
+    return ((int64_t)2 * w + (start > w * chunk ? 1 : 0)) * ROWS + x;
+  };
+  float top = kNegInf;
+  for (int w = w0; w <= w1; ++w) top = fmaxf(top, t.part_lse[at(w)]);
+  const float ref = is_neg_inf(top) ? 0.f : top;
+  constexpr int NV = DC / 256;
+  f32x4 acc[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = f32x4{};
+  float sum = 0.f;
+  for (int w = w0; w <= w1; ++w) {
+    const int64_t s = at(w);
+    const float g = fast_exp2(t.part_lse[s] - ref);   // NaN stays NaN
+    sum += g;
+    const float* src = t.part_o + s * DC + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] += *reinterpret_cast<const f32x4*>(src + 256 * i) * g;
+  }
+  const float ks = p.k_scale ? *p.k_scale : 1.f;
+  const float inv = empty_sum(sum) ? 0.f : ks / sum;
+  char* out = reinterpret_cast<char*>(p.out) + (o + 4 * lane) * out_bytes(p.out_dt);
+  auto put = [&](auto dtc) {
+    constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store_out4<DT>(out + 256 * i * ES, acc[i] * inv);
+  };
+  if (p.out_dt == QMLA_DT_F32) put(std::integral_constant<int, QMLA_DT_F32>{});
+  else if (p.out_dt == QMLA_DT_F16) put(std::integral_constant<int, QMLA_DT_F16>{});
+  else put(std::integral_constant<int, QMLA_DT_BF16>{});
+  if (lane == 0 && p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, row_lse(top, sum));
+}
+
+struct Inst {
+  bool fp8;
+  int d_c, rope_max, rows;
+  const void* fn;
+  const void* combine;
+  int (*lds)(int heads);
+};
+
+#define QMLA_TR(FP8, DC, CP, NS, ST) \
+  {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST>>, \
+   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST>>(heads); }}
+static const Inst kInst[] = {
+    QMLA_TR(true, 512, 576, 1, 2),  QMLA_TR(false, 512, 576, 1, 2),
+    QMLA_TR(true, 256, 512, 1, 2),  QMLA_TR(false, 256, 512, 1, 2),
+    QMLA_TR(true, 768, 1024, 2, 2), QMLA_TR(false, 768, 1024, 2, 2),
+    QMLA_TR(true, 1792, 2048, 4, 1), QMLA_TR(false, 1792, 2048, 4, 1),
+};
+
+static const Inst* find(const qmla_decode_params* p) {
+  for (const Inst& i : kInst)
+    if (i.fp8 == (p->kv_dtype == QMLA_KV_FP8) && i.d_c == p->d_c && p->rope_w <= i.rope_max && p->heads <= MAXH &&
+        i.lds(p->heads) <= LDS_MAX)
+      return &i;
+  return nullptr;
+}
+
+struct Layout {
+  size_t lse_off, o_off, total;
+  int nwg;
+};
+static Layout layout(const qmla_decode_params* p, const Inst& in) {
+  Layout l;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  l.nwg = p->num_workgroups > 0 ? p->num_workgroups : cu_count();
+  const int64_t n_req = p->rows / p->qrows;
+  l.lse_off = up((size_t)(1 + n_req) * 8);
+  l.o_off = l.lse_off + up((size_t)2 * l.nwg * in.rows * 4);
+  l.total = l.o_off + (size_t)2 * l.nwg * in.rows * p->d_c * 4;
+  return l;
+}
+
+}  // namespace tr
+}  // namespace qmla
+
+using namespace qmla;
+
+extern "C" {
+
+size_t qmla_tree_workspace_bytes(const qmla_decode_params* p) {
+  if (!p || p->rows <= 0 || p->qrows <= 0 || p->rows % p->qrows) return 0;
+  const tr::Inst* in = tr::find(p);
+  return in ? tr::layout(p, *in).total : 0;
+}
+
+int qmla_tree_forward(const qmla_decode_params* p0, const int64_t* tree_mask, int64_t mask_stride, const int32_t* node_counts,
+                      void* stream) {
+  if (!p0) return QMLA_ERR_NULL;
+  qmla_decode_params p = *p0;
+  p.num_splits = 1;
+  const int rc = validate_params(&p);
+  if (rc) return rc;
+  if (p.groups != 1 || p.qrows > 64 || p.num_workgroups < 0) return QMLA_ERR_SHAPE;
+  if (!rows16(&p)) return QMLA_ERR_ALIGN;
+  const int eb = p.kv_dtype == QMLA_KV_FP8 ? 1 : 2;
+  // the last load of a row may reach past its columns, never past its 16-byte multiple
+  if ((p.page_size > 1 ? p.token_stride : p.page_stride) * eb < ((int64_t)(p.d_c + p.rope_w) * eb + 15) / 16 * 16) return QMLA_ERR_SHAPE;
+  const tr::Inst* in = tr::find(&p);
+  if (!in) return QMLA_ERR_NOKERNEL;
+  if (p.rows == 0) return QMLA_OK;
+  if (!tree_mask) return QMLA_ERR_NULL;
+  if ((uintptr_t)tree_mask % 8) return QMLA_ERR_ALIGN;
+  const int64_t n_req = p.rows / p.qrows;
+  if (n_req > 65535) return QMLA_ERR_SHAPE;
+  const tr::Layout l = tr::layout(&p, *in);
+  if (!p.workspace || p.workspace_bytes < l.total) return QMLA_ERR_WORKSPACE;
+  if ((uintptr_t)p.workspace % 16) return QMLA_ERR_ALIGN;
+  tr::TrParams t{};
+  t.k = make_kparams(&p);
+  t.mask = tree_mask;
+  t.mask_sr = mask_stride;
+  t.counts = node_counts;
+  t.rows = p.qrows * p.heads;
+  t.rt = (t.rows + in->rows - 1) / in->rows;
+  t.cols = p.d_c + p.rope_w;
+  t.nwg = l.nwg;
+  t.min_chunk = 2;
+  t.rms_mode = p.rms_mode;
+  t.rms_b = p.rms_mode == QMLA_RMS_BF16 || p.rms_mode == QMLA_RMS_BF16_BYTES ? 2 : 1;
+  char* ws = reinterpret_cast<char*>(p.workspace);
+  t.plan = reinterpret_cast<int64_t*>(ws);
+  t.part_lse = reinterpret_cast<float*>(ws + l.lse_off);
+  t.part_o = reinterpret_cast<float*>(ws + l.o_off);
+  const int bytes = in->lds(p.heads);
+  if (hipFuncSetAttribute(in->fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return QMLA_ERR_LAUNCH;
+  void* args[] = {&t};
+  if (hipLaunchKernel(in->fn, dim3(t.nwg), dim3(tr::NT), args, bytes, (hipStream_t)stream) != hipSuccess) return QMLA_ERR_LAUNCH;
+  const hipError_t e = hipLaunchKernel(in->combine, dim3((in->rows + 3) / 4, t.rt, (unsigned)n_req), dim3(256), args, 0, (hipStream_t)stream);
+  return e == hipSuccess ? QMLA_OK : QMLA_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -180,11 +180,81 @@ class PrepParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of `qmla_rotary_params` (include/qmla.h); field order and types must match."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_token_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_token_stride", ctypes.c_int64),
+        ("k_out_head_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("pos_stride", ctypes.c_int64),
+        ("cos_sin", ctypes.c_void_p),
+        ("max_pos", ctypes.c_int64),
+        ("cos_sin_stride", ctypes.c_int64),
+        ("n", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("offset", ctypes.c_int32),
+        ("rot", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class EvictParams(ctypes.Structure):
+    """Mirror of `qmla_evict_params` (include/qmla.h); field order and types must match."""
+
+    _fields_ = [
+        ("weights", ctypes.c_void_p),
+        ("weights_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("index_stride", ctypes.c_int64),
+        ("counts", ctypes.c_void_p),
+        ("requests", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("keep", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("cache", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("row_bytes", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride", ctypes.c_int64),
+        ("bt_cols", ctypes.c_int32),
+        ("dst_block_table", ctypes.c_void_p),
+        ("dst_bt_stride", ctypes.c_int64),
+        ("dst_bt_cols", ctypes.c_int32),
+        ("first", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p),
+        ("weights_out_stride", ctypes.c_int64),
+        ("weights_out_width", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 # every function include/qmla.h declares, with its ctypes signature
 _P = ctypes.POINTER(DecodeParams)
 _W = ctypes.POINTER(CacheWriteParams)
 _G = ctypes.POINTER(GatherParams)
 _R = ctypes.POINTER(PrepParams)
+_T = ctypes.POINTER(RotaryParams)
+_E = ctypes.POINTER(EvictParams)
 SIGNATURES = {
     "qmla_version": (ctypes.c_int, []),
     "qmla_build_info": (ctypes.c_char_p, []),
@@ -199,6 +269,13 @@ SIGNATURES = {
     "qmla_cache_write": (ctypes.c_int, [_W, ctypes.c_void_p]),
     "qmla_gather": (ctypes.c_int, [_G, ctypes.c_void_p]),
     "qmla_prep": (ctypes.c_int, [_R, ctypes.c_void_p]),
+    "qmla_rotary": (ctypes.c_int, [_T, ctypes.c_void_p]),
+    "qmla_evict_select": (ctypes.c_int, [_E, ctypes.c_void_p]),
+    "qmla_cache_compact": (ctypes.c_int, [_E, ctypes.c_void_p]),
+    "qmla_attention_weights": (ctypes.c_int, [_P, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p]),
+    "qmla_tree_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "qmla_tree_forward": (ctypes.c_int, [_P, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 _lib = None
@@ -256,6 +333,14 @@ def as_scale(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype == torch.float32 and t.device == device:
         return t
     return t.reshape(-1)[:1].to(device=device, dtype=torch.float32).contiguous()
+
+
+def same_device(fn: str, **tensors) -> None:
+    """Every tensor given lives on the current GPU, where the launch goes."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is not None and (dev is None or t.device != dev):
+            raise ValueError(f"{fn}: {name} must live on the current GPU, got {t.device}")
 
 
 def check(fn: str, code: int) -> None:
