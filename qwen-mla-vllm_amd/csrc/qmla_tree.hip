@@ -49,6 +49,18 @@ __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// The score products name VGPRs: the output accumulators take every AGPR, and left to itself the compiler
+// accumulates scores there too, spilling what they displace (all 36 query fragments, reloaded each tile). The
+// compiler sees no matrix instruction in these statements, so the wait before their result is read is their
+// own: 24 states, more than the longest 32x32 product needs.
+__device__ __forceinline__ void mfma32_v0(f32x16& d, const bf16x8& a, const bf16x8& b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma32_v(f32x16& d, const bf16x8& a, const bf16x8& b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_v_done(f32x16& d) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(d)); }
+
 __device__ __forceinline__ int node_count(const TrParams& t, int b) {
   const int n = t.counts ? t.counts[b] : t.k.qrows;
   return n < 0 ? 0 : n < t.k.qrows ? n : t.k.qrows;
@@ -146,17 +158,28 @@ struct Cfg {
   static constexpr int OB = DC / NS / 32;          // output column blocks of a wave
   static constexpr int UC = FP8 ? 16 : 8;          // columns of a 16-byte load
   static constexpr int UPR = CP / UC;              // loads of a row
-  static constexpr int LOADS = (TT * UPR + NT - 1) / NT;
+  static constexpr int LOADS = (UPR + 7) / 8;      // loads of a thread
   static constexpr int TILE_B = TT * CP * 2;
   static_assert(DC % (32 * NS) == 0 && CP % (16 * NS) == 0 && CP % 64 == 0);
 };
 
+constexpr int KD = 6, VD = 5;   // LDS reads ahead of a score product, fragments ahead of a value product
+constexpr int RL = 2;         // dwords of divisors a thread loads ahead
 constexpr int IRS = TT + 4;   // floats of a head's divisors in LDS
 
 template <class C>
 __host__ __device__ constexpr int lds_bytes(int heads) {
-  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 2 * TT * 8 + 16;
+  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 4 * TT * 8 + 16;
 }
+
+typedef __attribute__((address_space(3))) char lchar;
+
+// One piece's constant state of a lane, and what it holds of the running softmax.
+struct Row {
+  int head, base, nodes;
+  uint64_t sees;
+  float m_ref, l_sum, l_p;
+};
 
 template <class C>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_kernel(const TrParams t) {
@@ -165,11 +188,11 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const int rg = wave / C::NS, cp = wave % C::NS;
-  char* kt = lds;
+  lchar* const kt = QMLA_LDS(char, lds);
   float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [STAGES][heads][IRS]
   char* part = lds + C::STAGES * (C::TILE_B + p.heads * IRS * 4);        // [4 waves][4][64] 16 bytes
-  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [2][TT]
-  uint32_t* odd = reinterpret_cast<uint32_t*>(rowoff + 2 * TT);          // [3], bit per token
+  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [4][TT]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(rowoff + 4 * TT);          // [4], bit per token
   // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
   const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   const Range rng = unit_range(t, w, w == 0);
@@ -177,6 +200,21 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   const float ks = p.k_scale ? *p.k_scale : 1.f;
   const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
   int bad = 0;
+  // this lane's reads of a staged tile. A tile and its rows lie on multiples of a swizzle group, so the chunk's
+  // low bits go onto an address with one exclusive or and the rest into the instruction's offset: score chunk
+  // 2f + h of row n, and the value fragment of columns 32 ob .. in rows 16 k2 + 8 x + vr
+  constexpr int NSW = C::RS % 32 == 0 ? 5 : C::RS % 32 == 16 ? 4 : 3;   // bits the swizzle flips
+  constexpr int GM = (1 << NSW) - 1;
+  static_assert((C::QC / 8) % 2 == 0 && (C::DC / C::NS / 8) % 4 == 0);
+  const int kc0 = cp * (C::QC / 8), vc0 = cp * (C::DC / C::NS / 8);
+  const uint32_t klane = n * (C::CP * 2) + ((swz<C::RS>(n) ^ h) << 4);
+  const int vq = lane & 15, vr = 4 * h + (vq >> 2), vc = 2 * ((lane >> 4) & 1) + ((vq & 3) >> 1);
+  uint32_t vlane[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) vlane[x] = (8 * x + vr) * (C::CP * 2) + ((swz<C::RS>(8 * x + vr) ^ vc) << 4) + (vq & 1) * 8;
+  // staging: 8 threads a row, loads 8 units apart
+  const int srow = tid >> 3, sc0 = tid & 7;
+  const uint32_t slane = srow * (C::CP * 2) + (((C::FP8 ? 2 * sc0 : sc0) ^ swz<C::RS>(srow)) << 4);
   int64_t u = rng.lo, c0 = rng.c0;
   int b = rng.b;
   while (u < rng.hi) {
@@ -195,27 +233,28 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     const bool rvalid = r < t.rows;
     const int node = rvalid ? r / p.heads : 0, head = rvalid ? r - node * p.heads : 0;
     const bool rlive = rvalid && node < nodes;
-    const uint64_t sees = rlive ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
     bf16x8 qf[C::NQ];
     {
+      // rows may be aligned to their elements only
+      typedef bf16x8 bf16x8_e __attribute__((aligned(2)));
       const int64_t row = (int64_t)b * p.qrows + node;
       const __bf16* qn = p.q_nope + row * p.qn_sr + head * p.qn_sh;
       const __bf16* qp = p.q_pe + row * p.qp_sr + head * p.qp_sh;
+      const int whole8 = p.rope_w & ~7;
+      bf16x8 tail{};
+      for (int i = 0; i < (p.rope_w & 7); ++i) {
+        const __bf16 x = qp[whole8 + i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tail[e] = e == i ? x : tail[e];
+      }
 #pragma unroll
       for (int f = 0; f < C::NQ; ++f) {
-        const int c = cp * C::QC + 16 * f + 8 * h;
-        bf16x8 v{};
-        if (rlive) {
-          if (c < C::DC) {
-            v = load_q8(qn + c, p.q_vec);
-          } else if (c - C::DC + 8 <= p.rope_w) {
-            v = load_q8(qp + (c - C::DC), p.q_vec);
-          } else {
+        const int c = cp * C::QC + 16 * f + 8 * h, o = c - C::DC;
+        bf16x8 v = tail;
+        if (o < 0) v = *reinterpret_cast<const bf16x8_e*>(qn + c);
+        else if (o < whole8) v = *reinterpret_cast<const bf16x8_e*>(qp + o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c - C::DC + i < p.rope_w) v[i] = qp[c - C::DC + i];
-          }
-        }
+        for (int e = 0; e < 8; ++e) v[e] = rlive && o <= whole8 ? v[e] : (__bf16)0.f;
         qf[f] = v;
       }
     }
@@ -226,8 +265,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 
     // ---- staging
     i32x4 raw[C::LOADS];
-    constexpr int RL = MAXH * TT / NT;
     uint32_t rraw[RL];
+    const int rd0 = p.rms_off_b >> 2, rskip = p.rms_off_b & 3;           // the divisors' first dword, bytes before them
+    const int rdw = t.rms_mode == QMLA_RMS_NONE ? 0 : (rskip + p.heads * t.rms_b + 3) >> 2;
     auto rows_of = [&](int j) {   // byte offsets of tile j's rows
       if (tid < TT) {
         const int tok = j * TT + tid;
@@ -237,97 +277,250 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           const int id = checked_page(p, p.bt[b * p.bt_stride + pg], bad);
           off = id * p.page_stride_b + (int64_t)(tok - pg * p.page_size) * p.token_stride_b;
         }
-        rowoff[(j & 1) * TT + tid] = off;
+        rowoff[(j & 3) * TT + tid] = off;
       }
     };
     auto fetch = [&](int j) {
+      const int64_t off_now = rowoff[(j & 3) * TT + srow];
+      const char* src = p.kv + (off_now >= 0 ? off_now : 0) + 16 * sc0;
 #pragma unroll
       for (int i = 0; i < C::LOADS; ++i) {
-        const int q = i * NT + tid, row = q / C::UPR, c = q % C::UPR;
         raw[i] = i32x4{};
-        if (q < TT * C::UPR) {
-          const int64_t off = rowoff[(j & 1) * TT + row];
-          if (off >= 0 && c * C::UC < t.cols) raw[i] = *reinterpret_cast<const i32x4*>(p.kv + off + 16 * c);
-        }
+        if (off_now >= 0 && (sc0 + 8 * i) * C::UC < t.cols) raw[i] = *reinterpret_cast<const i32x4*>(src + 128 * i);
       }
 #pragma unroll
       for (int i = 0; i < RL; ++i) {
-        const int q = i * NT + tid;
         rraw[i] = 0;
-        if ((q >> 5) < p.heads && t.rms_mode != QMLA_RMS_NONE) {
-          const int64_t off = rowoff[(j & 1) * TT + (q & 31)];
-          if (off >= 0) {
-            const uint8_t* at = reinterpret_cast<const uint8_t*>(p.kv + off + p.rms_off_b + (q >> 5) * t.rms_b);
-            rraw[i] = t.rms_b == 2 ? at[0] | ((uint32_t)at[1] << 8) : at[0];
-          }
-        }
+        if (off_now >= 0 && sc0 + 8 * i < rdw) rraw[i] = *reinterpret_cast<const uint32_t*>(p.kv + off_now + 4 * (rd0 + sc0 + 8 * i));
+      }
+    };
+    auto put_rms = [&](float* o, int d, uint32_t v) {   // dword d of a row's divisors
+      if (t.rms_b == 1) {
+        const int hd = 4 * d - rskip;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((uint32_t)(hd + e) < (uint32_t)p.heads) o[(hd + e) * IRS] = fs * inv_divisor((v >> (8 * e)) & 0xff, t.rms_mode, ks);
+      } else {
+        // an odd byte offset splits a divisor over two dwords: those rows have theirs read by bytes below
+        const int hd = 2 * d - (rskip >> 1);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if ((uint32_t)(hd + e) < (uint32_t)p.heads) o[(hd + e) * IRS] = fs * inv_divisor((v >> (16 * e)) & 0xffff, t.rms_mode, ks);
       }
     };
     auto put = [&](int j) {
-      char* dst = kt + (C::STAGES > 1 ? (j & 1) * C::TILE_B : 0);
-      const bool drafted = (j + 1) * TT > base;
+      lchar* dst = kt + (j % C::STAGES) * C::TILE_B;
+      if (t.cols % C::UC) {   // the divisors begin inside a load
 #pragma unroll
-      for (int i = 0; i < C::LOADS; ++i) {
-        const int q = i * NT + tid, row = q / C::UPR, c = q % C::UPR;
-        if (q < TT * C::UPR) {
-          i32x4 v = raw[i];
-          const int left = t.cols - c * C::UC;
-          if (left < C::UC) {   // the divisors begin inside this load
+        for (int i = 0; i < C::LOADS; ++i) {
+          const int left = t.cols - (sc0 + 8 * i) * C::UC;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const int bits = left * (C::FP8 ? 8 : 16) - 32 * d;
-              v[d] = bits <= 0 ? 0 : bits >= 32 ? v[d] : v[d] & (int)((1u << bits) - 1);
-            }
-          }
-          if (drafted && j * TT + row >= base && any_odd<C::FP8>(v)) {
-            atomicOr(&odd[j % 3], 1u << row);
-            v = i32x4{};
-          }
-          const int s = swz<C::RS>(row);
-          char* at = dst + row * (C::CP * 2);
-          if constexpr (C::FP8) {
-            bf16x8 x, y;
-            fp8x16_to_bf16(v, x, y);
-            *reinterpret_cast<bf16x8*>(at + (((2 * c) ^ s) << 4)) = x;
-            *reinterpret_cast<bf16x8*>(at + (((2 * c + 1) ^ s) << 4)) = y;
-          } else {
-            *reinterpret_cast<i32x4*>(at + ((c ^ s) << 4)) = v;
+          for (int d = 0; d < 4; ++d) {
+            const int bits = left * (C::FP8 ? 8 : 16) - 32 * d;
+            raw[i][d] = bits <= 0 ? 0 : bits >= 32 ? raw[i][d] : raw[i][d] & (int)((1u << (bits & 31)) - 1);
           }
         }
       }
-      float* ir = irms + (C::STAGES > 1 ? (j & 1) * p.heads * IRS : 0);
+      if ((j + 1) * TT > base) {   // drafted tokens: what is not finite goes into `odd`
+        bool any = false;
 #pragma unroll
-      for (int i = 0; i < RL; ++i) {
-        const int q = i * NT + tid;
-        if ((q >> 5) < p.heads) ir[(q >> 5) * IRS + (q & 31)] = fs * inv_divisor(rraw[i], t.rms_mode, ks);
+        for (int i = 0; i < C::LOADS; ++i) {
+          const bool o = j * TT + srow >= base && any_odd<C::FP8>(raw[i]);
+          any = any || o;
+          raw[i] = o ? i32x4{} : raw[i];
+        }
+        if (any) atomicOr(&odd[j & 3], 1u << srow);
       }
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i) {
+        if (C::UPR % 8 == 0 || i + 1 < C::LOADS || sc0 < C::UPR % 8) {
+          constexpr int per = C::FP8 ? 16 : 8;   // chunks from load to load
+          const uint32_t at = ((uint32_t)(uintptr_t)dst + slane) ^ (((per * i) & GM) << 4);
+          typedef __attribute__((address_space(3))) bf16x8 lvec;
+          constexpr int hi = 0;
+          (void)hi;
+          if constexpr (C::FP8) {
+            bf16x8 x, y;
+            fp8x16_to_bf16(raw[i], x, y);
+            *(lvec*)(uintptr_t)(at + (((per * i) & ~GM) << 4)) = x;
+            *(lvec*)(uintptr_t)((at ^ 16) + (((per * i) & ~GM) << 4)) = y;
+          } else {
+            *(lvec*)(uintptr_t)(at + (((per * i) & ~GM) << 4)) = __builtin_bit_cast(bf16x8, raw[i]);
+          }
+        }
+      }
+      float* ir = irms + (j % C::STAGES) * p.heads * IRS + srow;
+      if (t.rms_mode == QMLA_RMS_NONE) {
+        for (int hd = sc0; hd < p.heads; hd += 8) ir[hd * IRS] = fs;
+      } else if (t.rms_b == 2 && (rskip & 1)) {
+        for (int hd = sc0; hd < p.heads; hd += 8) {
+          const int64_t off_put = rowoff[(j & 3) * TT + srow];
+          const uint8_t* at = reinterpret_cast<const uint8_t*>(p.kv + off_put + p.rms_off_b + 2 * hd);
+          ir[hd * IRS] = off_put >= 0 ? fs * inv_divisor(at[0] | ((uint32_t)at[1] << 8), t.rms_mode, ks) : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < RL; ++i)
+          if (sc0 + 8 * i < rdw) put_rms(ir, sc0 + 8 * i, rraw[i]);
+        // many heads: the rest of the divisors without a step's head start
+        for (int d = sc0 + 8 * RL; d < rdw; d += 8) {
+          const int64_t off_put = rowoff[(j & 3) * TT + srow];
+          put_rms(ir, d, off_put >= 0 ? *reinterpret_cast<const uint32_t*>(p.kv + off_put + 4 * (rd0 + d)) : 0);
+        }
+      }
+    };
+    // ---- scores of tile j. One wave a SIMD: nothing but this order hides the LDS, so a slot of one product
+    // issues the read KD products ahead, and nothing moves between slots
+    auto score = [&](int j, f32x16& s) {
+      const uint32_t src = (uint32_t)(uintptr_t)(kt + (j % C::STAGES) * C::TILE_B) + klane + (kc0 << 4);
+      typedef __attribute__((address_space(3))) const bf16x8 lvec;
+      auto read = [&](int f) { return *(lvec*)(uintptr_t)((src ^ (((2 * f) & GM) << 4)) + (((2 * f) & ~GM) << 4)); };
+      bf16x8 k[KD];
+#pragma unroll
+      for (int f = 0; f < KD; ++f) k[f] = read(f);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = 0; f < C::NQ; ++f) {
+        const bf16x8 a = k[f % KD];
+        if (f + KD < C::NQ) k[f % KD] = read(f + KD);
+        if (f == 0) mfma32_v0(s, a, qf[f]);
+        else mfma32_v(s, a, qf[f]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      mfma_v_done(s);
+    };
+    // ---- divide, cap, mask
+    auto finish = [&](int j, f32x16& s) {
+      const float* ir = irms + (j % C::STAGES) * p.heads * IRS + head * IRS + 4 * h;
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
+      }
+      if (p.logit_cap > 0.f) {
+        const float in = 2.0f * kLog2e / p.logit_cap, out = p.logit_cap * kLog2e;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = out - 2.0f * out * __builtin_amdgcn_rcpf(fast_exp2(s[i] * in) + 1.0f);
+      }
+      if ((j + 1) * TT > base) {
+        const uint32_t od = odd[j & 3];
+        const uint64_t sees = rlive ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
+          const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
+          s[i] = !vis ? kNegInf : (od >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
+        }
+      }
+    };
+    // ---- softmax against a reference that moves when a row's maximum has passed it by kMoveAt (a row's own
+    // doing: what its neighbours hold does not move it; a NaN maximum moves nothing)
+    auto value_read = [&](uint32_t src, int i) {   // fragment i: columns 32 (i / 2) .., tokens 16 (i % 2) ..
+      typedef short i16x8 __attribute__((ext_vector_type(8)));
+      i16x4 v[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int c = (C::NS > 1 ? vc0 : 0) + 4 * (i >> 1);
+        const uint32_t at = ((src + vlane[2 * (i & 1) + x]) ^ ((c & GM) << 4)) + ((c & ~GM) << 4);
+        v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(uintptr_t)at);
+      }
+      const i16x8 va = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+      return __builtin_bit_cast(bf16x8, va);
+    };
+    // values of tile j against P, `beside(i)` in the slot of product i
+    auto values = [&](int j, const bf16x8 (&pf)[2], auto&& beside) {
+      const uint32_t src = (uint32_t)(uintptr_t)(kt + (j % C::STAGES) * C::TILE_B);
+      bf16x8 v[VD];
+#pragma unroll
+      for (int i = 0; i < VD; ++i) v[i] = value_read(src, i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2 * C::OB; ++i) {
+        const bf16x8 a = v[i % VD];
+        if (i + VD < 2 * C::OB) v[i % VD] = value_read(src, i + VD);
+        acc[i >> 1] = mfma32(a, pf[i & 1], acc[i >> 1]);
+        beside(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // the softmax of s in steps 0 .. NSOFT - 1, small enough to lie beside one product each
+    struct Soft {
+      float mx, m_use, m_new, es, ep;
+    } sf;
+    auto soft_step = [&](int i, f32x16& s, bf16x8 (&pn)[2]) {
+      if (i == 0) {
+        sf.mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+        sf.es = sf.ep = 0.f;
+      } else if (i < 6) {
+        sf.mx = fmaxf(fmaxf(sf.mx, s[2 * i + 1]), s[2 * i + 2]);
+      } else if (i == 6) {
+        sf.mx = fmaxf(fmaxf(sf.mx, s[13]), fmaxf(s[14], s[15]));
+      } else if (i == 7) {
+        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sf.mx), __float_as_uint(sf.mx), false, false);
+        sf.mx = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+        sf.m_new = sf.mx > m_ref + kMoveAt ? sf.mx : m_ref;
+        sf.m_use = is_neg_inf(sf.m_new) ? 0.f : sf.m_new;
+      } else if (i < 16) {
+        const int x = 2 * (i - 8);
+        s[x] = fast_exp2(s[x] - sf.m_use);
+        s[x + 1] = fast_exp2(s[x + 1] - sf.m_use);
+      } else if (i < 24) {
+        const int x = 2 * (i - 16);
+        sf.es += s[x] + s[x + 1];
+        const bf16x2 e{(__bf16)s[x], (__bf16)s[x + 1]};
+        pn[x >> 3][x & 7] = e[0];
+        pn[x >> 3][(x & 7) + 1] = e[1];
+        sf.ep = __builtin_amdgcn_fdot2_f32_bf16(e, bf16x2{(__bf16)1.f, (__bf16)1.f}, sf.ep, false);
+      }
+    };
+    constexpr int NSOFT = 24;
+    auto rescale = [&](float m_new, float es, float ep) {
+      const bool moves = m_new != m_ref;
+      if (__builtin_amdgcn_ballot_w64(moves)) {
+        const float alpha = moves ? fast_exp2(m_ref - m_new) : 1.f;
+        l_sum *= alpha;
+        l_p *= alpha;
+#pragma unroll
+        for (int ob = 0; ob < C::OB; ++ob) {
+          // one block at a time, there and back: left to the compiler all of them pass through VGPRs at
+          // once and displace the queries
+          asm volatile("" : "+a"(acc[ob]));
+          acc[ob] *= alpha;
+          asm volatile("" : "+a"(acc[ob]));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        m_ref = m_new;
+      }
+      l_sum += es;
+      l_p += ep;
     };
 
     __syncthreads();   // the last piece's tiles are read
-    if (tid < 3) odd[tid] = 0;
+    if (tid < 4) odd[tid] = 0;
     rows_of(ta);
+    if (ta + 1 < te) rows_of(ta + 1);
     __syncthreads();
     fetch(ta);
-    if (ta + 1 < te) rows_of(ta + 1);
     put(ta);
+    if (ta + 1 < te) fetch(ta + 1);
     __syncthreads();
+    if (ta + 2 < te) rows_of(ta + 2);
 
+    // step j: tile j's scores and softmax beside tile j-1's values (three stages), or before its own; tile
+    // j+1 goes into LDS, j+2's loads start. A wave without rows stages only.
+    constexpr bool PIPE = C::STAGES >= 3;
+    bf16x8 pf[2] = {};
     for (int j = ta; j < te; ++j) {
-      const char* src = kt + (C::STAGES > 1 ? (j & 1) * C::TILE_B : 0);
-      if (j + 1 < te) fetch(j + 1);
-      if (j + 2 < te) rows_of(j + 2);
-      if (tid == 0) odd[(j + 2) % 3] = 0;
-      // ---- scores
-      f32x16 s{};
-      if (wlive) {
-        const char* krow = src + n * (C::CP * 2);
-        const int sw = swz<C::RS>(n);
-#pragma unroll
-        for (int f = 0; f < C::NQ; ++f) {
-          const int c = cp * (C::QC / 8) + 2 * f + h;
-          s = mfma32(*reinterpret_cast<const bf16x8*>(krow + ((c ^ sw) << 4)), qf[f], s);
-        }
+      __syncthreads();
+      if (tid == 0) odd[(j + 2) & 3] = 0;
+      if constexpr (C::STAGES > 1) {
+        if (j + 1 < te) put(j + 1);
+        if (j + 2 < te) fetch(j + 2);
       }
+      if (j + 3 < te) rows_of(j + 3);
+      f32x16 s{};
+      if (wlive) score(j, s);
       if constexpr (C::NS > 1) {
         if (wlive) {
 #pragma unroll
@@ -348,82 +541,33 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         }
       }
       if (wlive) {
-        // ---- divide, cap, mask
-        const float* ir = irms + (C::STAGES > 1 ? (j & 1) * p.heads * IRS : 0) + head * IRS + 4 * h;
+        finish(j, s);
+        bf16x8 pn[2];
+        if constexpr (PIPE) {
+          // (a piece's first step has no tile before it: zeros against its own)
+          static_assert(2 * C::OB >= NSOFT || 2 * C::OB == 16);
+          constexpr int PER = 2 * C::OB >= NSOFT ? 1 : 2;   // softmax steps a slot
+          values(j > ta ? j - 1 : j, pf, [&](int i) {
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
+            for (int x = 0; x < PER; ++x) soft_step(PER * i + x, s, pn);
+          });
+          rescale(sf.m_new, sf.es, sf.ep);
+          pf[0] = pn[0];
+          pf[1] = pn[1];
+        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
-        }
-        if (p.logit_cap > 0.f) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[i] = p.logit_cap * kLog2e * (1.0f - 2.0f / (fast_exp2(2.0f * kLog2e * (s[i] / p.logit_cap)) + 1.0f));
-        }
-        if ((j + 1) * TT > base) {
-          const uint32_t od = odd[j % 3];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
-            const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
-            s[i] = !vis ? kNegInf : (od >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
-          }
-        }
-        // ---- softmax against a reference that moves when a row's maximum has passed it by kMoveAt
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        {
-          const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          mx = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-        }
-        // (a row's own doing: what its neighbours hold does not move it; a NaN maximum moves nothing)
-        const bool moves = mx > m_ref + kMoveAt;
-        if (__builtin_amdgcn_ballot_w64(moves)) {
-          const float alpha = moves ? fast_exp2(m_ref - mx) : 1.f;
-          l_sum *= alpha;
-          l_p *= alpha;
-#pragma unroll
-          for (int ob = 0; ob < C::OB; ++ob) acc[ob] *= alpha;
-          m_ref = moves ? mx : m_ref;
-        }
-        const float m_use = is_neg_inf(m_ref) ? 0.f : m_ref;
-        bf16x8 pf[2];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = fast_exp2(s[i] - m_use);
-          l_sum += e;
-          const __bf16 e16 = (__bf16)e;
-          l_p += (float)e16;
-          pf[i >> 3][i & 7] = e16;
-        }
-        // ---- values
-        {
-          const int q = lane & 15, rr = 4 * h + (q >> 2);
-#pragma unroll
-          for (int ob = 0; ob < C::OB; ++ob) {
-            const int col = cp * (C::DC / C::NS) + 32 * ob + 16 * ((lane >> 4) & 1) + 4 * (q & 3);
-#pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              i16x4 v[2];
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int row = 16 * k2 + 8 * x + rr;
-                const char* at = src + row * (C::CP * 2) + (((col >> 3) ^ swz<C::RS>(row)) << 4) + (col & 4) * 2;
-                v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(QMLA_LDS(i16x4, at));
-              }
-              typedef short i16x8 __attribute__((ext_vector_type(8)));
-              const i16x8 va = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-              acc[ob] = mfma32(__builtin_bit_cast(bf16x8, va), pf[k2], acc[ob]);
-            }
-          }
+          for (int i = 0; i < NSOFT; ++i) soft_step(i, s, pn);
+          rescale(sf.m_new, sf.es, sf.ep);
+          values(j, pn, [](int) {});
         }
       }
-      if constexpr (C::STAGES == 1) __syncthreads();
-      if (j + 1 < te) put(j + 1);
-      __syncthreads();
+      if constexpr (C::STAGES == 1) {
+        __syncthreads();
+        if (j + 1 < te) put(j + 1);
+        if (j + 2 < te) fetch(j + 2);
+      }
     }
+    if (PIPE && wlive) values(te - 1, pf, [](int) {});
 
     // ---- this piece's rows
     if (wlive && rvalid) {
@@ -451,6 +595,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
             store_out4<DT>(ob0 + (32 * ob + 8 * i4) * ES, v);
+            __builtin_amdgcn_sched_barrier(0);
           }
       };
       if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
@@ -531,8 +676,8 @@ struct Inst {
   {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST>>, \
    (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST>>(heads); }}
 static const Inst kInst[] = {
-    QMLA_TR(true, 512, 576, 1, 2),  QMLA_TR(false, 512, 576, 1, 2),
-    QMLA_TR(true, 256, 512, 1, 2),  QMLA_TR(false, 256, 512, 1, 2),
+    QMLA_TR(true, 512, 576, 1, 3),  QMLA_TR(false, 512, 576, 1, 3),
+    QMLA_TR(true, 256, 512, 1, 3),  QMLA_TR(false, 256, 512, 1, 3),
     QMLA_TR(true, 768, 1024, 2, 2), QMLA_TR(false, 768, 1024, 2, 2),
     QMLA_TR(true, 1792, 2048, 4, 1), QMLA_TR(false, 1792, 2048, 4, 1),
 };
