@@ -51,13 +51,14 @@ __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const
 
 // The score products name VGPRs: the output accumulators take every AGPR, and left to itself the compiler
 // accumulates scores there too, spilling what they displace (all 36 query fragments, reloaded each tile). The
-// compiler sees no matrix instruction in these statements, so the wait before their result is read is their
-// own: 24 states, more than the longest 32x32 product needs.
+// compiler sees no matrix instruction in these statements, so the waits are their own: two states after a vector
+// instruction that may have written an operand (a copy the allocator placed; they pass behind the last product),
+// and 24 before the result is read, more than the longest 32x32 product needs.
 __device__ __forceinline__ void mfma32_v0(f32x16& d, const bf16x8& a, const bf16x8& b) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mfma32_v(f32x16& d, const bf16x8& a, const bf16x8& b) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+  asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mfma_v_done(f32x16& d) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(d)); }
 
@@ -148,10 +149,11 @@ __device__ __forceinline__ bool any_odd(const i32x4& v) {
   return odd;
 }
 
-template <bool FP8_, int DC_, int CP_, int NS_, int STAGES_>
+template <bool FP8_, int DC_, int CP_, int NS_, int STAGES_, int QL_>
 struct Cfg {
   static constexpr bool FP8 = FP8_;
   static constexpr int DC = DC_, CP = CP_, NS = NS_, STAGES = STAGES_;
+  static constexpr int QL = QL_;                   // a wave's last query fragments, kept in LDS
   static constexpr int ROWS = 128 / NS;            // query rows of a workgroup
   static constexpr int RS = CP / 8;                // 16-byte chunks of a staged row
   static constexpr int QC = CP / NS, NQ = QC / 16; // score columns of a wave, its products
@@ -163,13 +165,13 @@ struct Cfg {
   static_assert(DC % (32 * NS) == 0 && CP % (16 * NS) == 0 && CP % 64 == 0);
 };
 
-constexpr int KD = 6, VD = 5;   // LDS reads ahead of a score product, fragments ahead of a value product
+constexpr int KD = 5, VD = 4;   // LDS reads ahead of a score product, fragments ahead of a value product
 constexpr int RL = 2;         // dwords of divisors a thread loads ahead
 constexpr int IRS = TT + 4;   // floats of a head's divisors in LDS
 
 template <class C>
 __host__ __device__ constexpr int lds_bytes(int heads) {
-  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 4 * TT * 8 + 16;
+  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 4 * C::QL * 1024 + 4 * TT * 8 + 16;
 }
 
 typedef __attribute__((address_space(3))) char lchar;
@@ -191,7 +193,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   lchar* const kt = QMLA_LDS(char, lds);
   float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [STAGES][heads][IRS]
   char* part = lds + C::STAGES * (C::TILE_B + p.heads * IRS * 4);        // [4 waves][4][64] 16 bytes
-  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [4][TT]
+  char* ql = part + (C::NS > 1 ? 4 * 4096 : 0);                          // [4 waves][QL][64] 16 bytes
+  int64_t* rowoff = reinterpret_cast<int64_t*>(ql + 4 * C::QL * 1024);   // [4][TT]
   uint32_t* odd = reinterpret_cast<uint32_t*>(rowoff + 4 * TT);          // [4], bit per token
   // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
   const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
@@ -212,9 +215,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   uint32_t vlane[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x) vlane[x] = (8 * x + vr) * (C::CP * 2) + ((swz<C::RS>(8 * x + vr) ^ vc) << 4) + (vq & 1) * 8;
-  // staging: 8 threads a row, loads 8 units apart
-  const int srow = tid >> 3, sc0 = tid & 7;
-  const uint32_t slane = srow * (C::CP * 2) + (((C::FP8 ? 2 * sc0 : sc0) ^ swz<C::RS>(srow)) << 4);
   int64_t u = rng.lo, c0 = rng.c0;
   int b = rng.b;
   while (u < rng.hi) {
@@ -228,15 +228,24 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     const int te = rng.hi - u < nt - ta ? ta + (int)(rng.hi - u) : nt;
     const int L = p.seq_lens[b], nodes = node_count(t, b), base = L - nodes;
     // ---- this lane's query row
-    const int r0 = m * C::ROWS + rg * 32, r = r0 + n;
+    // Of the thread only what the tile loop uses is kept over it: the rest is worked out again where it is
+    // needed (`own` keeps the compiler from doing so ahead). Held, it would push other values into scratch, whose
+    // reloads wait for every load in flight.
+    auto own = [&]() {
+      int x = tid;
+      asm volatile("" : "+v"(x));
+      return x;
+    };
+    const int r0 = m * C::ROWS + rg * 32;
     const bool wlive = r0 < t.rows;
-    const bool rvalid = r < t.rows;
-    const int node = rvalid ? r / p.heads : 0, head = rvalid ? r - node * p.heads : 0;
-    const bool rlive = rvalid && node < nodes;
-    bf16x8 qf[C::NQ];
+    int irms_at;   // this row's head in the divisors
+    bf16x8 qf[C::NQ - C::QL];
+    char* const qlw = ql + (wave * C::QL * 64 + lane) * 16;
     {
       // rows may be aligned to their elements only
       typedef bf16x8 bf16x8_e __attribute__((aligned(2)));
+      const int r = r0 + n < t.rows ? r0 + n : t.rows - 1, node = r / p.heads, head = r - node * p.heads;
+      irms_at = head * IRS + 4 * h;
       const int64_t row = (int64_t)b * p.qrows + node;
       const __bf16* qn = p.q_nope + row * p.qn_sr + head * p.qn_sh;
       const __bf16* qp = p.q_pe + row * p.qp_sr + head * p.qp_sh;
@@ -249,13 +258,21 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
 #pragma unroll
       for (int f = 0; f < C::NQ; ++f) {
+        // dead rows keep what they read: their columns of the products go nowhere
         const int c = cp * C::QC + 16 * f + 8 * h, o = c - C::DC;
-        bf16x8 v = tail;
-        if (o < 0) v = *reinterpret_cast<const bf16x8_e*>(qn + c);
-        else if (o < whole8) v = *reinterpret_cast<const bf16x8_e*>(qp + o);
+        if (C::NS == 1 && 16 * f < C::DC) {
+          if (f < C::NQ - C::QL) qf[f] = *reinterpret_cast<const bf16x8_e*>(qn + c);
+          else *reinterpret_cast<bf16x8*>(qlw + (f - (C::NQ - C::QL)) * 1024) = *reinterpret_cast<const bf16x8_e*>(qn + c);
+        } else {
+          bf16x8 v = tail;
+          if (o < 0) v = *reinterpret_cast<const bf16x8_e*>(qn + c);
+          else if (o < whole8) v = *reinterpret_cast<const bf16x8_e*>(qp + o);
+          i32x4 x = __builtin_bit_cast(i32x4, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = rlive && o <= whole8 ? v[e] : (__bf16)0.f;
-        qf[f] = v;
+          for (int e = 0; e < 4; ++e) x[e] = o <= whole8 ? x[e] : 0;
+          if (f < C::NQ - C::QL) qf[f] = __builtin_bit_cast(bf16x8, x);
+          else *reinterpret_cast<i32x4*>(qlw + (f - (C::NQ - C::QL)) * 1024) = x;
+        }
       }
     }
     f32x16 acc[C::OB];
@@ -268,30 +285,45 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     uint32_t rraw[RL];
     const int rd0 = p.rms_off_b >> 2, rskip = p.rms_off_b & 3;           // the divisors' first dword, bytes before them
     const int rdw = t.rms_mode == QMLA_RMS_NONE ? 0 : (rskip + p.heads * t.rms_b + 3) >> 2;
-    auto rows_of = [&](int j) {   // byte offsets of tile j's rows
+    // byte offsets of tile j's rows, in two steps: a thread's page id, and a step later its row. The id is
+    // loaded before the step's rows are, so the wait for the last step's rows covers it.
+    int pid = 0;
+    auto page_of = [&](int j) {
+      const int tok = j * TT + tid;
+      if (tid < TT && tok < L) pid = p.bt[b * p.bt_stride + page_div(p, tok)];
+    };
+    auto rows_of = [&](int j) {
       if (tid < TT) {
         const int tok = j * TT + tid;
         int64_t off = -1;
-        if (tok < L) {
-          const int pg = page_div(p, tok);
-          const int id = checked_page(p, p.bt[b * p.bt_stride + pg], bad);
-          off = id * p.page_stride_b + (int64_t)(tok - pg * p.page_size) * p.token_stride_b;
-        }
+        if (tok < L) off = checked_page(p, pid, bad) * p.page_stride_b + (int64_t)(tok - page_div(p, tok) * p.page_size) * p.token_stride_b;
         rowoff[(j & 3) * TT + tid] = off;
       }
     };
+    // Loads of tile j's rows. Rows past the request read the cache's first row and loads past a row's units its
+    // first unit; put() drops both.
     auto fetch = [&](int j) {
-      const int64_t off_now = rowoff[(j & 3) * TT + srow];
-      const char* src = p.kv + (off_now >= 0 ? off_now : 0) + 16 * sc0;
+      const int me = own(), row = me >> 3, c = me & 7;
+      const int64_t off = rowoff[(j & 3) * TT + row];
+      const char* src = p.kv + (off >= 0 ? off : 0);
+      if (t.cols == C::CP) {
 #pragma unroll
-      for (int i = 0; i < C::LOADS; ++i) {
-        raw[i] = i32x4{};
-        if (off_now >= 0 && (sc0 + 8 * i) * C::UC < t.cols) raw[i] = *reinterpret_cast<const i32x4*>(src + 128 * i);
+        for (int i = 0; i < C::LOADS; ++i) {
+          const bool past = C::UPR % 8 != 0 && i + 1 == C::LOADS && c >= C::UPR % 8;
+          raw[i] = *reinterpret_cast<const i32x4*>(src + (past ? 0 : 16 * c + 128 * i));
+        }
+      } else {
+        int cols = t.cols;
+        asm volatile("" : "+s"(cols));
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i)
+          raw[i] = *reinterpret_cast<const i32x4*>(src + ((c + 8 * i) * C::UC < cols ? 16 * c + 128 * i : 0));
       }
+      if (rdw > 0) {
+        const char* rs = src + 4 * rd0;
 #pragma unroll
-      for (int i = 0; i < RL; ++i) {
-        rraw[i] = 0;
-        if (off_now >= 0 && sc0 + 8 * i < rdw) rraw[i] = *reinterpret_cast<const uint32_t*>(p.kv + off_now + 4 * (rd0 + sc0 + 8 * i));
+        for (int i = 0; i < RL; ++i)
+          if (8 * i < rdw) rraw[i] = *reinterpret_cast<const uint32_t*>(rs + 4 * (c + 8 * i < rdw ? c + 8 * i : 0));
       }
     };
     auto put_rms = [&](float* o, int d, uint32_t v) {   // dword d of a row's divisors
@@ -309,11 +341,15 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
     };
     auto put = [&](int j) {
-      lchar* dst = kt + (j % C::STAGES) * C::TILE_B;
-      if (t.cols % C::UC) {   // the divisors begin inside a load
+      const int me = own(), row = me >> 3, sc0 = me & 7;
+      const uint32_t slane = (uint32_t)(uintptr_t)(kt + (j % C::STAGES) * C::TILE_B) + row * (C::CP * 2) +
+                             (((C::FP8 ? 2 * sc0 : sc0) ^ swz<C::RS>(row)) << 4);
+      if (t.cols != C::CP) {   // columns past the row's keys
+        int cols = t.cols;
+        asm volatile("" : "+s"(cols));
 #pragma unroll
         for (int i = 0; i < C::LOADS; ++i) {
-          const int left = t.cols - (sc0 + 8 * i) * C::UC;
+          const int left = cols - (sc0 + 8 * i) * C::UC;
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             const int bits = left * (C::FP8 ? 8 : 16) - 32 * d;
@@ -321,24 +357,24 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           }
         }
       }
-      if ((j + 1) * TT > base) {   // drafted tokens: what is not finite goes into `odd`
+      if ((j + 1) * TT > base) {   // rows past the request; drafted tokens: what is not finite goes into `odd`
+        const int tok = j * TT + row;
         bool any = false;
 #pragma unroll
         for (int i = 0; i < C::LOADS; ++i) {
-          const bool o = j * TT + srow >= base && any_odd<C::FP8>(raw[i]);
-          any = any || o;
-          raw[i] = o ? i32x4{} : raw[i];
+          const bool o = tok >= base && any_odd<C::FP8>(raw[i]);
+          const bool past = C::UPR % 8 != 0 && i + 1 == C::LOADS && sc0 >= C::UPR % 8;
+          any = any || (o && !past);
+          raw[i] = o || tok >= L ? i32x4{} : raw[i];
         }
-        if (any) atomicOr(&odd[j & 3], 1u << srow);
+        if (any && tok < L) atomicOr(&odd[j & 3], 1u << row);
       }
 #pragma unroll
       for (int i = 0; i < C::LOADS; ++i) {
         if (C::UPR % 8 == 0 || i + 1 < C::LOADS || sc0 < C::UPR % 8) {
           constexpr int per = C::FP8 ? 16 : 8;   // chunks from load to load
-          const uint32_t at = ((uint32_t)(uintptr_t)dst + slane) ^ (((per * i) & GM) << 4);
+          const uint32_t at = slane ^ (((per * i) & GM) << 4);
           typedef __attribute__((address_space(3))) bf16x8 lvec;
-          constexpr int hi = 0;
-          (void)hi;
           if constexpr (C::FP8) {
             bf16x8 x, y;
             fp8x16_to_bf16(raw[i], x, y);
@@ -349,12 +385,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           }
         }
       }
-      float* ir = irms + (j % C::STAGES) * p.heads * IRS + srow;
+      float* ir = irms + (j % C::STAGES) * p.heads * IRS + row;
       if (t.rms_mode == QMLA_RMS_NONE) {
         for (int hd = sc0; hd < p.heads; hd += 8) ir[hd * IRS] = fs;
       } else if (t.rms_b == 2 && (rskip & 1)) {
         for (int hd = sc0; hd < p.heads; hd += 8) {
-          const int64_t off_put = rowoff[(j & 3) * TT + srow];
+          const int64_t off_put = rowoff[(j & 3) * TT + row];
           const uint8_t* at = reinterpret_cast<const uint8_t*>(p.kv + off_put + p.rms_off_b + 2 * hd);
           ir[hd * IRS] = off_put >= 0 ? fs * inv_divisor(at[0] | ((uint32_t)at[1] << 8), t.rms_mode, ks) : 0.f;
         }
@@ -364,7 +400,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           if (sc0 + 8 * i < rdw) put_rms(ir, sc0 + 8 * i, rraw[i]);
         // many heads: the rest of the divisors without a step's head start
         for (int d = sc0 + 8 * RL; d < rdw; d += 8) {
-          const int64_t off_put = rowoff[(j & 3) * TT + srow];
+          const int64_t off_put = rowoff[(j & 3) * TT + row];
           put_rms(ir, d, off_put >= 0 ? *reinterpret_cast<const uint32_t*>(p.kv + off_put + 4 * (rd0 + d)) : 0);
         }
       }
@@ -375,7 +411,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       const uint32_t src = (uint32_t)(uintptr_t)(kt + (j % C::STAGES) * C::TILE_B) + klane + (kc0 << 4);
       typedef __attribute__((address_space(3))) const bf16x8 lvec;
       auto read = [&](int f) { return *(lvec*)(uintptr_t)((src ^ (((2 * f) & GM) << 4)) + (((2 * f) & ~GM) << 4)); };
-      bf16x8 k[KD];
+      bf16x8 k[KD], q[C::QL > 0 ? C::QL : 1];
+      const uint32_t qsrc = (uint32_t)(uintptr_t)QMLA_LDS(char, qlw);
 #pragma unroll
       for (int f = 0; f < KD; ++f) k[f] = read(f);
       __builtin_amdgcn_sched_barrier(0);
@@ -384,14 +421,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         const bf16x8 a = k[f % KD];
         if (f + KD < C::NQ) k[f % KD] = read(f + KD);
         if (f == 0) mfma32_v0(s, a, qf[f]);
-        else mfma32_v(s, a, qf[f]);
+        else if (f < C::NQ - C::QL) mfma32_v(s, a, qf[f]);
+        else mfma32_v(s, a, q[f - (C::NQ - C::QL)]);
+        constexpr int Q0 = C::NQ - C::QL - KD;   // the queries in LDS as far ahead
+        if (f >= Q0 && f < Q0 + C::QL) q[f - Q0] = *(lvec*)(uintptr_t)(qsrc + (f - Q0) * 1024);
         __builtin_amdgcn_sched_barrier(0);
       }
       mfma_v_done(s);
     };
     // ---- divide, cap, mask
     auto finish = [&](int j, f32x16& s) {
-      const float* ir = irms + (j % C::STAGES) * p.heads * IRS + head * IRS + 4 * h;
+      const float* ir = irms + (j % C::STAGES) * p.heads * IRS + irms_at;
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
@@ -405,7 +445,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
       if ((j + 1) * TT > base) {
         const uint32_t od = odd[j & 3];
-        const uint64_t sees = rlive ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
+        const int r = m * C::ROWS + rg * 32 + (own() & 31), node = r / p.heads;
+        const uint64_t sees = r < t.rows && node < nodes ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
@@ -498,14 +539,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 
     __syncthreads();   // the last piece's tiles are read
     if (tid < 4) odd[tid] = 0;
-    rows_of(ta);
-    if (ta + 1 < te) rows_of(ta + 1);
+    // (rows past the piece's end but inside the request are looked up and not fetched)
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      page_of(ta + x);
+      rows_of(ta + x);
+    }
+    page_of(ta + 3);
     __syncthreads();
     fetch(ta);
     put(ta);
     if (ta + 1 < te) fetch(ta + 1);
-    __syncthreads();
-    if (ta + 2 < te) rows_of(ta + 2);
 
     // step j: tile j's scores and softmax beside tile j-1's values (three stages), or before its own; tile
     // j+1 goes into LDS, j+2's loads start. A wave without rows stages only.
@@ -516,9 +560,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       if (tid == 0) odd[(j + 2) & 3] = 0;
       if constexpr (C::STAGES > 1) {
         if (j + 1 < te) put(j + 1);
+      }
+      rows_of(j + 3);
+      page_of(j + 4);
+      if constexpr (C::STAGES > 1) {
         if (j + 2 < te) fetch(j + 2);
       }
-      if (j + 3 < te) rows_of(j + 3);
       f32x16 s{};
       if (wlive) score(j, s);
       if constexpr (C::NS > 1) {
@@ -570,14 +617,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     if (PIPE && wlive) values(te - 1, pf, [](int) {});
 
     // ---- this piece's rows
-    if (wlive && rvalid) {
+    const int me = own(), n = me & 31, h = (me >> 5) & 1;
+    const int r = r0 + n;
+    if (r < t.rows) {
+      const int node = r / p.heads, head = r - node * p.heads;
       {
         const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_sum), __float_as_uint(l_sum), false, false);
         l_sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
         const auto o2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_p), __float_as_uint(l_p), false, false);
         l_p = __uint_as_float(o2[0]) + __uint_as_float(o2[1]);
       }
-      if (!rlive) l_sum = l_p = 0.f;
+      if (node >= nodes) l_sum = l_p = 0.f;
       const bool whole = ta == 0 && te == nt;
       const int64_t slot = 2 * w + (u > rng.lo ? 1 : 0);
       const float inv = empty_sum(l_p) ? 0.f : (whole ? ks : 1.f) / l_p;
@@ -672,14 +722,14 @@ struct Inst {
   int (*lds)(int heads);
 };
 
-#define QMLA_TR(FP8, DC, CP, NS, ST) \
-  {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST>>, \
-   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST>>(heads); }}
+#define QMLA_TR(FP8, DC, CP, NS, ST, QL) \
+  {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST, QL>>, \
+   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST, QL>>(heads); }}
 static const Inst kInst[] = {
-    QMLA_TR(true, 512, 576, 1, 3),  QMLA_TR(false, 512, 576, 1, 3),
-    QMLA_TR(true, 256, 512, 1, 3),  QMLA_TR(false, 256, 512, 1, 3),
-    QMLA_TR(true, 768, 1024, 2, 2), QMLA_TR(false, 768, 1024, 2, 2),
-    QMLA_TR(true, 1792, 2048, 4, 1), QMLA_TR(false, 1792, 2048, 4, 1),
+    QMLA_TR(true, 512, 576, 1, 3, 4),   QMLA_TR(false, 512, 576, 1, 3, 4),
+    QMLA_TR(true, 256, 512, 1, 3, 0),   QMLA_TR(false, 256, 512, 1, 3, 0),
+    QMLA_TR(true, 768, 1024, 2, 2, 0),  QMLA_TR(false, 768, 1024, 2, 2, 0),
+    QMLA_TR(true, 1792, 2048, 4, 1, 0), QMLA_TR(false, 1792, 2048, 4, 1, 0),
 };
 
 static const Inst* find(const qmla_decode_params* p) {
