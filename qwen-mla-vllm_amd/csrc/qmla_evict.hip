@@ -30,11 +30,16 @@ __device__ __forceinline__ uint32_t order(float w) {
 constexpr int NT = 1024, NW = NT / 64;
 constexpr int BITS = 11, BINS = 1 << BITS;   // digits of 11, 11 and 10 bits
 
+constexpr int KEYS = 36 * 1024;               // keys LDS holds beside the histogram
+
 // One workgroup a request: the m-th largest key of the middle tokens by three digit histograms, then one
 // pass that counts per wave and one that writes. Waves take contiguous runs, so ranks among equal keys
-// and output places follow from per-wave counts without a barrier per run.
+// and output places follow from per-wave counts without a barrier per run. KEPT: the keys stay in LDS after
+// the first pass (a request of up to KEYS tokens), else every pass reads the weights again.
+template <bool KEPT>
 __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
   const qmla_evict_params& p = e.p;
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ uint32_t hist[BINS];
   __shared__ uint32_t sh_digit, sh_need;
   __shared__ int wave_eq[NW], wave_gt[NW], wave_sum[NW];
@@ -52,6 +57,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
   for (int i = tid; i < lo; i += NT) index[i] = i;
   for (int i = tid; i < p.recent; i += NT) index[lo + m + i] = hi + i;
   if (m == 0) return;
+  auto key = [&](int t) { return KEPT ? keys[t - lo] : order(w[t]); };
   // key of rank m among the middle tokens: prefix holds its decided high bits
   uint32_t prefix = 0, need = (uint32_t)m;
   int shift = 32;
@@ -60,31 +66,22 @@ __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
     shift -= bits;
     for (int i = tid; i < BINS; i += NT) hist[i] = 0;
     __syncthreads();
-    for (int base = lo; base < hi; base += 4 * NT) {
-      uint32_t k[4];
+    constexpr int G = 8;
+    for (int base = lo; base < hi; base += G * NT) {
+      uint32_t k[G];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < G; ++q) {
         const int t = base + q * NT + tid;
-        k[q] = t < hi ? order(w[t]) : 0;
+        k[q] = 0;
+        if (t < hi) k[q] = d == 0 ? order(w[t]) : key(t);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < G; ++q) {
         const int t = base + q * NT + tid;
+        if (KEPT && d == 0 && t < hi) keys[t - lo] = k[q];
         const bool in = t < hi && (d == 0 || (k[q] >> (shift + bits)) == prefix);
         const uint32_t digit = (k[q] >> shift) & ((1u << bits) - 1);
-        // equal digits of a wave (weights repeat: many tokens never got any) go in one addition, up to
-        // twice; what is left adds by itself
-        uint64_t live = __builtin_amdgcn_ballot_w64(in);
-#pragma unroll
-        for (int rep = 0; rep < 2; ++rep) {
-          if (!live) break;
-          const int lead = __builtin_ctzll(live);
-          const uint32_t ld = (uint32_t)__builtin_amdgcn_readlane((int)digit, lead);
-          const uint64_t same = __builtin_amdgcn_ballot_w64(((live >> lane) & 1) && digit == ld);
-          if (lane == lead) atomicAdd(&hist[ld], (uint32_t)__builtin_popcountll(same));
-          live &= ~same;
-        }
-        if ((live >> lane) & 1) atomicAdd(&hist[digit], 1u);
+        if (in) atomicAdd(&hist[digit], 1u);
       }
     }
     __syncthreads();
@@ -119,7 +116,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int t = base + 64 * q + lane;
-      const uint32_t k = t < r1 ? order(w[t]) : 0;
+      const uint32_t k = t < r1 ? key(t) : 0;
       gt += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t < r1 && k > prefix));
       eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t < r1 && k == prefix));
     }
@@ -137,7 +134,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
   }
   for (int base = r0; base < r1; base += 64) {
     const int t = base + lane;
-    const uint32_t k = t < r1 ? order(w[t]) : 0;
+    const uint32_t k = t < r1 ? key(t) : 0;
     const uint64_t me = __builtin_amdgcn_ballot_w64(t < r1 && k == prefix);
     const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(me >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)me, 0));
     const bool take = t < r1 && (k > prefix || (k == prefix && eq0 + below < (int)need));
@@ -169,25 +166,46 @@ __device__ __forceinline__ int64_t row_at(const EParams& e, const int* table, in
   return id * p.page_stride + (int64_t)(tok - pg * p.page_size) * p.token_stride;
 }
 
-// Out of place: a thread copies one unit of one row; blockIdx.y is the request.
+// Out of place: a thread copies MU units of its request's rows, a workgroup's width apart; blockIdx.y is the
+// request.
+constexpr int MU = 1;
 template <class V>
 __global__ __launch_bounds__(256) void move_kernel(const EParams e) {
   const qmla_evict_params& p = e.p;
   const int b = blockIdx.y;
   const int n = min(max(p.counts[b], 0), p.keep);
-  const uint32_t u = blockIdx.x * 256u + threadIdx.x;
-  const int i = (int)magic_div(u, e.chunk_mul, e.chunk_sh), c = (int)u - i * e.chunks;
-  if (i >= n) return;
-  int bad = 0;
-  const int tok = p.index[b * p.index_stride + i], to = (p.first ? p.first[b] : 0) + i;
-  const int64_t s = row_at(e, p.block_table, p.bt_stride, p.bt_cols, b, tok, bad);
-  const int64_t d = row_at(e, p.dst_block_table, p.dst_bt_stride, p.dst_bt_cols, b, to, bad);
-  if (s >= 0 && d >= 0) *((V*)((char*)p.cache + d) + c) = *((const V*)((const char*)p.cache + s) + c);
-  if (c == 0) {
-    if (p.weights_out && (uint32_t)tok < (uint32_t)p.width && (uint32_t)to < (uint32_t)p.weights_out_width)
-      p.weights_out[b * p.weights_out_stride + to] = p.weights[b * p.weights_stride + tok];
-    if (bad && p.status) *p.status = QMLA_ERR_PAGE;
+  const uint32_t u0 = blockIdx.x * (256u * MU) + threadIdx.x;
+  if (u0 - threadIdx.x >= (uint32_t)n * (uint32_t)e.chunks) return;
+  const int first = p.first ? p.first[b] : 0;
+  int bad = 0, i[MU], c[MU], tok[MU];
+  int64_t s[MU], d[MU];
+#pragma unroll
+  for (int q = 0; q < MU; ++q) {
+    const uint32_t u = u0 + 256u * q;
+    i[q] = (int)magic_div(u, e.chunk_mul, e.chunk_sh);
+    c[q] = (int)u - i[q] * e.chunks;
+    tok[q] = i[q] < n ? p.index[b * p.index_stride + i[q]] : -1;
   }
+#pragma unroll
+  for (int q = 0; q < MU; ++q) {
+    s[q] = d[q] = -1;
+    if (i[q] < n) {
+      s[q] = row_at(e, p.block_table, p.bt_stride, p.bt_cols, b, tok[q], bad);
+      d[q] = row_at(e, p.dst_block_table, p.dst_bt_stride, p.dst_bt_cols, b, first + i[q], bad);
+    }
+  }
+  V v[MU];
+#pragma unroll
+  for (int q = 0; q < MU; ++q)
+    if (s[q] >= 0 && d[q] >= 0) v[q] = __builtin_nontemporal_load((const V*)((const char*)p.cache + s[q]) + c[q]);
+#pragma unroll
+  for (int q = 0; q < MU; ++q) {
+    if (s[q] >= 0 && d[q] >= 0) __builtin_nontemporal_store(v[q], (V*)((char*)p.cache + d[q]) + c[q]);
+    const int to = first + i[q];
+    if (i[q] < n && c[q] == 0 && p.weights_out && (uint32_t)tok[q] < (uint32_t)p.width && (uint32_t)to < (uint32_t)p.weights_out_width)
+      p.weights_out[b * p.weights_out_stride + to] = p.weights[b * p.weights_stride + tok[q]];
+  }
+  if (bad && p.status) *p.status = QMLA_ERR_PAGE;
 }
 
 // In place: one workgroup owns CW units of every row of a request (blockIdx.x names them; the last
@@ -269,7 +287,14 @@ int qmla_evict_select(const qmla_evict_params* p, void* stream) {
   ev::EParams e{};
   e.p = *p;
   void* args[] = {&e};
-  const hipError_t r = hipLaunchKernel((const void*)&ev::select_kernel, dim3(p->requests), dim3(ev::NT), args, 0, (hipStream_t)stream);
+  // the middle tokens of the longest request
+  const int64_t most = (int64_t)p->width - p->sink - p->recent;
+  const bool kept = most <= ev::KEYS;
+  const int bytes = kept && most > 0 ? (int)most * 4 : 0;
+  const void* fn = kept ? (const void*)&ev::select_kernel<true> : (const void*)&ev::select_kernel<false>;
+  if (bytes > 48 * 1024 && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return QMLA_ERR_LAUNCH;
+  const hipError_t r = hipLaunchKernel(fn, dim3(p->requests), dim3(ev::NT), args, bytes, (hipStream_t)stream);
   return r == hipSuccess ? QMLA_OK : QMLA_ERR_LAUNCH;
 }
 
@@ -290,12 +315,12 @@ int qmla_cache_compact(const qmla_evict_params* p, void* stream) {
   page_magic(p->page_size, e.page_mul, e.page_sh);
   page_magic(e.chunks, e.chunk_mul, e.chunk_sh);
   const bool in_place = !p->dst_block_table;
-  if ((int64_t)p->keep * e.chunks > 0x7fffffff - 256) return QMLA_ERR_SHAPE;
+  if ((int64_t)p->keep * e.chunks > 0x7fffffff - 256 * ev::MU) return QMLA_ERR_SHAPE;
   const void* fn = v == 16  ? (in_place ? (const void*)&ev::move_in_place_kernel<i32x4> : (const void*)&ev::move_kernel<i32x4>)
                    : v == 4 ? (in_place ? (const void*)&ev::move_in_place_kernel<int> : (const void*)&ev::move_kernel<int>)
                    : v == 2 ? (in_place ? (const void*)&ev::move_in_place_kernel<short> : (const void*)&ev::move_kernel<short>)
                             : (in_place ? (const void*)&ev::move_in_place_kernel<char> : (const void*)&ev::move_kernel<char>);
-  const uint32_t gx = in_place ? (e.chunks + ev::CW - 1) / ev::CW + 1 : ((int64_t)p->keep * e.chunks + 255) / 256;
+  const uint32_t gx = in_place ? (e.chunks + ev::CW - 1) / ev::CW + 1 : ((int64_t)p->keep * e.chunks + 256 * ev::MU - 1) / (256 * ev::MU);
   void* args[] = {&e};
   const hipError_t r = hipLaunchKernel(fn, dim3(gx, p->requests), dim3(in_place ? ev::NT : 256), args, 0, (hipStream_t)stream);
   return r == hipSuccess ? QMLA_OK : QMLA_ERR_LAUNCH;

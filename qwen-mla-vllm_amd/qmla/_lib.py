@@ -335,12 +335,19 @@ def as_scale(t: torch.Tensor, device) -> torch.Tensor:
     return t.reshape(-1)[:1].to(device=device, dtype=torch.float32).contiguous()
 
 
-def same_device(fn: str, **tensors) -> None:
-    """Every tensor given lives on the current GPU, where the launch goes."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else None
-    for name, t in tensors.items():
-        if t is not None and (dev is None or t.device != dev):
-            raise ValueError(f"{fn}: {name} must live on the current GPU, got {t.device}")
+def same_device(fn: str, *tensors) -> None:
+    """Every tensor given (name, tensor or None, ...) lives on the current GPU, where the launch goes."""
+    here = -1
+    for i in range(1, len(tensors), 2):
+        t = tensors[i]
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{fn}: {tensors[i - 1]} must live on the GPU, got {t.device}")
+        if here < 0:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise ValueError(f"{fn}: {tensors[i - 1]} must live on the current GPU, got {t.device}")
 
 
 def check(fn: str, code: int) -> None:

@@ -14,9 +14,9 @@ from . import _lib
 from .decode import _kv_code, _rms_mode, build_params
 
 
-def _rows32(name: str, t: torch.Tensor, dtype, dim: int) -> None:
-    if t.dtype != dtype or t.dim() != dim or (t.numel() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise TypeError(f"{name} must be a {dim}-D {dtype} tensor with contiguous rows")
+def _rows32(fn: str, name: str, t: torch.Tensor, dtype, dim: int) -> None:
+    if t.dtype is not dtype or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel() > 0):
+        raise TypeError(f"{fn}: {name} must be a {dim}-D {dtype} tensor with contiguous rows")
 
 
 def attention_weights(q_nope, q_rope, kv_cache, block_table, seq_lens, lse, weights, *, d_c=None, rope_w=None,
@@ -34,15 +34,16 @@ def attention_weights(q_nope, q_rope, kv_cache, block_table, seq_lens, lse, weig
         raise ValueError(f"attention_weights: rows {rows} not a multiple of qrows {qrows}")
     n_req = rows // qrows
     out = weights if out is None else out
-    _rows32("attention_weights: weights", weights, torch.float32, 2)
-    _rows32("attention_weights: out", out, torch.float32, 2)
-    _rows32("attention_weights: lse", lse, torch.float32, 2)
+    _rows32("attention_weights", "weights", weights, torch.float32, 2)
+    _rows32("attention_weights", "out", out, torch.float32, 2)
+    _rows32("attention_weights", "lse", lse, torch.float32, 2)
     if weights.shape[0] != n_req or out.shape != weights.shape:
         raise ValueError(f"attention_weights: weights and out must be [{n_req}, width]")
     if tuple(lse.shape) != (rows, H) or block_table.shape[0] != rows or seq_lens.shape[0] != rows:
         raise ValueError("attention_weights: lse, block_table and seq_lens need one row per query row")
-    _lib.same_device("attention_weights", q_nope=q_nope, q_rope=q_rope, kv_cache=kv_cache, block_table=block_table,
-                     seq_lens=seq_lens, lse=lse, weights=weights, out=out, status=status)
+    _lib.same_device("attention_weights", "q_nope", q_nope, "q_rope", q_rope, "kv_cache", kv_cache,
+                     "block_table", block_table, "seq_lens", seq_lens, "lse", lse, "weights", weights, "out", out,
+                     "status", status)
     p = row_params(q_nope, q_rope, kv_cache, block_table, seq_lens, q_nope, None, d_c=d_c, rope_w=rope_w, rms_offset=rms_offset,
                    page_size=page_size, sm_scale=sm_scale, kv_fp8=kv_fp8, fp8_rms=fp8_rms, k_scale=k_scale, groups=groups,
                    rms_heads=rms_heads, logit_cap=logit_cap, status=status)
@@ -79,22 +80,22 @@ def row_params(q_nope, q_rope, kv_cache, block_table, seq_lens, out, lse, *, d_c
 
 
 def _select_params(weights, seq_lens, keep, sink, recent, index, counts):
-    _rows32("evict_select: weights", weights, torch.float32, 2)
-    _rows32("evict_select: seq_lens", seq_lens, torch.int32, 1)
+    _rows32("evict_select", "weights", weights, torch.float32, 2)
+    _rows32("evict_select", "seq_lens", seq_lens, torch.int32, 1)
     n = weights.shape[0]
     if seq_lens.shape[0] != n:
         raise ValueError("evict_select: one length per row of weights")
     if keep < 0 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("evict_select: sink and recent must fit in keep")
     if index is not None:
-        _rows32("evict_select: index", index, torch.int32, 2)
+        _rows32("evict_select", "index", index, torch.int32, 2)
         if tuple(index.shape) != (n, keep):
             raise ValueError(f"evict_select: index must be [{n}, {keep}]")
     if counts is not None:
-        _rows32("evict_select: counts", counts, torch.int32, 1)
+        _rows32("evict_select", "counts", counts, torch.int32, 1)
         if counts.shape[0] != n:
             raise ValueError(f"evict_select: counts must be [{n}]")
-    _lib.same_device("evict_select", weights=weights, seq_lens=seq_lens, index=index, counts=counts)
+    _lib.same_device("evict_select", "weights", weights, "seq_lens", seq_lens, "index", index, "counts", counts)
     if index is None:
         index = torch.empty(n, keep, dtype=torch.int32, device=weights.device)
     if counts is None:
@@ -139,25 +140,25 @@ def cache_compact(kv_cache, block_table, index, counts, *, first=None, dst_block
 def _compact_params(p, kv_cache, block_table, index, counts, first, dst_block_table, weights, weights_out, status) -> None:
     if kv_cache.dim() not in (3, 4) or (kv_cache.dim() == 4 and kv_cache.shape[2] != 1) or kv_cache.stride(-1) != 1:
         raise ValueError("cache_compact: kv_cache must be [num_pages, page_size, (1,) row] with contiguous rows")
-    _rows32("cache_compact: block_table", block_table, torch.int32, 2)
-    _rows32("cache_compact: index", index, torch.int32, 2)
-    _rows32("cache_compact: counts", counts, torch.int32, 1)
+    _rows32("cache_compact", "block_table", block_table, torch.int32, 2)
+    _rows32("cache_compact", "index", index, torch.int32, 2)
+    _rows32("cache_compact", "counts", counts, torch.int32, 1)
     n = index.shape[0]
     if block_table.shape[0] != n or counts.shape[0] != n:
         raise ValueError("cache_compact: block_table, index and counts need one row per request")
     if first is not None:
-        _rows32("cache_compact: first", first, torch.int32, 1)
+        _rows32("cache_compact", "first", first, torch.int32, 1)
         if first.shape[0] != n:
             raise ValueError("cache_compact: first needs one entry per request")
     if dst_block_table is not None:
-        _rows32("cache_compact: dst_block_table", dst_block_table, torch.int32, 2)
+        _rows32("cache_compact", "dst_block_table", dst_block_table, torch.int32, 2)
         if dst_block_table.shape[0] != n:
             raise ValueError("cache_compact: dst_block_table needs one row per request")
     if weights_out is not None:
         if weights is None:
             raise ValueError("cache_compact: weights_out without weights")
         for name, t in (("weights", weights), ("weights_out", weights_out)):
-            _rows32(f"cache_compact: {name}", t, torch.float32, 2)
+            _rows32("cache_compact", name, t, torch.float32, 2)
             if t.shape[0] != n:
                 raise ValueError(f"cache_compact: {name} needs one row per request")
         same = weights_out.data_ptr() == weights.data_ptr()
@@ -165,8 +166,9 @@ def _compact_params(p, kv_cache, block_table, index, counts, first, dst_block_ta
             raise ValueError("cache_compact: weights_out may be weights in place only")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise TypeError("cache_compact: status must be an int32 tensor")
-    _lib.same_device("cache_compact", kv_cache=kv_cache, block_table=block_table, index=index, counts=counts, first=first,
-                     dst_block_table=dst_block_table, weights=weights, weights_out=weights_out, status=status)
+    _lib.same_device("cache_compact", "kv_cache", kv_cache, "block_table", block_table, "index", index,
+                     "counts", counts, "first", first, "dst_block_table", dst_block_table, "weights", weights,
+                     "weights_out", weights_out, "status", status)
     es = kv_cache.element_size()
     p.index, p.index_stride, p.counts = index.data_ptr(), index.stride(0), counts.data_ptr()
     p.requests, p.keep = n, index.shape[1]

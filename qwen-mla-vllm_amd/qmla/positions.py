@@ -121,28 +121,32 @@ def rotary(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, cos
         raise TypeError("rotary: q and k must share dtype and head dim")
     if k is None and k_out is not None:
         raise ValueError("rotary: k_out without k")
-    _lib.same_device("rotary", positions=positions, q=q, k=k, cos_sin=cos_sin, q_out=q_out, k_out=k_out)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _check_out("q", q, q_out)
-    if k is not None:
-        _check_out("k", k, k_out)
+    _lib.same_device("rotary", "positions", positions, "q", q, "k", k, "cos_sin", cos_sin, "q_out", q_out,
+                     "k_out", k_out)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_out("q", q, q_out)
     keep = ()
     if positions.dtype != torch.int64:
         positions = positions.to(torch.int64)
         keep = (positions,)
     p = _lib.RotaryParams()
-    p.q, p.q_token_stride, p.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    p.q_out, p.q_out_token_stride, p.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    p.q, (p.q_token_stride, p.q_head_stride, _) = q.data_ptr(), q.stride()
+    p.q_out, (p.q_out_token_stride, p.q_out_head_stride, _) = q_out.data_ptr(), q_out.stride()
     if k is not None:
-        p.k, p.k_token_stride, p.k_head_stride = k.data_ptr(), k.stride(0), k.stride(1)
-        p.k_out, p.k_out_token_stride, p.k_out_head_stride = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        else:
+            _check_out("k", k, k_out)
+        p.k, (p.k_token_stride, p.k_head_stride, _) = k.data_ptr(), k.stride()
+        p.k_out, (p.k_out_token_stride, p.k_out_head_stride, _) = k_out.data_ptr(), k_out.stride()
         p.k_heads = k.shape[1]
     p.positions, p.pos_stride = positions.data_ptr(), positions.stride(0)
     p.cos_sin, p.max_pos, p.cos_sin_stride = cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.stride(0)
-    p.n, p.q_heads, p.head_dim, p.offset, p.rot = n, q.shape[1], q.shape[2], offset, rot
-    p.interleaved, p.inverse, p.dtype = int(layout == "interleaved"), int(inverse), _DT[q.dtype]
+    p.n, p.q_heads, p.head_dim = q.shape
+    p.offset, p.rot = offset, rot
+    p.interleaved, p.inverse, p.dtype = layout == "interleaved", inverse, _DT[q.dtype]
     _lib.check("qmla_rotary", _lib.lib().qmla_rotary(ctypes.byref(p), _lib.stream()))
     if keep:
         _lib.keep_alive(keep)

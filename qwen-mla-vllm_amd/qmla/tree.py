@@ -62,8 +62,9 @@ def tree_forward(q_nope, q_rope, kv_cache, block_table, seq_lens, tree_mask, *, 
     if node_counts is not None and (node_counts.dtype != torch.int32 or node_counts.dim() != 1 or node_counts.shape[0] != n_req
                                     or (n_req > 1 and node_counts.stride(0) != 1)):
         raise TypeError("tree_forward: node_counts must be [requests] int32, contiguous")
-    _lib.same_device("tree_forward", q_nope=q_nope, q_rope=q_rope, kv_cache=kv_cache, block_table=block_table,
-                     seq_lens=seq_lens, tree_mask=tree_mask, node_counts=node_counts, out=out, lse=lse, status=status)
+    _lib.same_device("tree_forward", "q_nope", q_nope, "q_rope", q_rope, "kv_cache", kv_cache,
+                     "block_table", block_table, "seq_lens", seq_lens, "tree_mask", tree_mask,
+                     "node_counts", node_counts, "out", out, "lse", lse, "status", status)
     dv = q_nope.shape[-1] if d_c is None else d_c
     if out is None:
         out = torch.empty(rows, H, dv, dtype=torch.bfloat16, device=q_nope.device)
@@ -81,7 +82,7 @@ def tree_forward(q_nope, q_rope, kv_cache, block_table, seq_lens, tree_mask, *, 
         ws = torch.empty(need, dtype=torch.uint8, device=q_nope.device) if workspace is None \
             else workspace.reserve(need, q_nope.device)
     else:
-        _lib.same_device("tree_forward", workspace=workspace)
+        _lib.same_device("tree_forward", "workspace", workspace)
         ws = workspace
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
     _lib.check("qmla_tree_forward", lib.qmla_tree_forward(p, tree_mask.data_ptr(), tree_mask.stride(0),
