@@ -176,12 +176,139 @@ __host__ __device__ constexpr int lds_bytes(int heads) {
 
 typedef __attribute__((address_space(3))) char lchar;
 
-// One piece's constant state of a lane, and what it holds of the running softmax.
-struct Row {
-  int head, base, nodes;
-  uint64_t sees;
-  float m_ref, l_sum, l_p;
+// ---- what the kernels share: a tile's scores of a lane's row to P, the running sums, a finished piece ------
+// divide by the divisors (ir: this row's, from LDS, scaled) and cap: log2-domain scores
+__device__ __forceinline__ void finish_scores(const TrParams& t, f32x16& s, const float* ir) {
+#pragma unroll
+  for (int i4 = 0; i4 < 4; ++i4) {
+    const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
+  }
+  const float cap = t.k.logit_cap;
+  if (cap > 0.f) {
+    const float in = 2.0f * kLog2e / cap, out = cap * kLog2e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = out - 2.0f * out * __builtin_amdgcn_rcpf(fast_exp2(s[i] * in) + 1.0f);
+  }
+}
+// a tile with drafted tokens: what the row's node does not see, and tokens with a bad element
+__device__ __forceinline__ void mask_scores(const TrParams& t, f32x16& s, int j, int b, int base, int nodes, int r0, int me,
+                                            uint32_t odd) {
+  const int r = r0 + (me & 31), node = r / t.k.heads, h = (me >> 5) & 1;
+  const uint64_t sees = r < t.rows && node < nodes ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
+    const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
+    s[i] = !vis ? kNegInf : (odd >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
+  }
+}
+
+// The softmax of s against a reference that moves when a row's maximum has passed it by kMoveAt (a row's own
+// doing: what its neighbours hold does not move it; a NaN maximum moves nothing), in steps 0 .. NSOFT - 1 small
+// enough to lie beside one product each.
+struct Soft {
+  float mx, m_use, m_new, es, ep;
 };
+constexpr int NSOFT = 24;
+__device__ __forceinline__ void soft_step(int i, f32x16& s, bf16x8 (&pn)[2], Soft& sf, float m_ref) {
+  if (i == 0) {
+    sf.mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+    sf.es = sf.ep = 0.f;
+  } else if (i < 6) {
+    sf.mx = fmaxf(fmaxf(sf.mx, s[2 * i + 1]), s[2 * i + 2]);
+  } else if (i == 6) {
+    sf.mx = fmaxf(fmaxf(sf.mx, s[13]), fmaxf(s[14], s[15]));
+  } else if (i == 7) {
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sf.mx), __float_as_uint(sf.mx), false, false);
+    sf.mx = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+    sf.m_new = sf.mx > m_ref + kMoveAt ? sf.mx : m_ref;
+    sf.m_use = is_neg_inf(sf.m_new) ? 0.f : sf.m_new;
+  } else if (i < 16) {
+    const int x = 2 * (i - 8);
+    s[x] = fast_exp2(s[x] - sf.m_use);
+    s[x + 1] = fast_exp2(s[x + 1] - sf.m_use);
+  } else if (i < 24) {
+    const int x = 2 * (i - 16);
+    sf.es += s[x] + s[x + 1];
+    const bf16x2 e{(__bf16)s[x], (__bf16)s[x + 1]};
+    pn[x >> 3][x & 7] = e[0];
+    pn[x >> 3][(x & 7) + 1] = e[1];
+    sf.ep = __builtin_amdgcn_fdot2_f32_bf16(e, bf16x2{(__bf16)1.f, (__bf16)1.f}, sf.ep, false);
+  }
+}
+template <int OB>
+__device__ __forceinline__ void rescale(const Soft& sf, float& m_ref, float& l_sum, float& l_p, f32x16 (&acc)[OB]) {
+  const bool moves = sf.m_new != m_ref;
+  if (__builtin_amdgcn_ballot_w64(moves)) {
+    const float alpha = moves ? fast_exp2(m_ref - sf.m_new) : 1.f;
+    l_sum *= alpha;
+    l_p *= alpha;
+#pragma unroll
+    for (int ob = 0; ob < OB; ++ob) {
+      // one block at a time, there and back: left to the compiler all of them pass through VGPRs at once and
+      // displace the queries
+      asm volatile("" : "+a"(acc[ob]));
+      acc[ob] *= alpha;
+      asm volatile("" : "+a"(acc[ob]));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    m_ref = sf.m_new;
+  }
+  l_sum += sf.es;
+  l_p += sf.ep;
+}
+
+// The rows of a finished piece: the final output and lse where it held all of the request's tokens, else
+// partial slot `slot`. me: the thread.
+struct Piece {
+  int b, m, nodes, rg, cp;
+  int64_t slot;
+  bool whole;
+};
+template <class C>
+__device__ __forceinline__ void store_piece(const TrParams& t, const Piece& q, int me, float ks, float m_ref, float l_sum,
+                                            float l_p, const f32x16 (&acc)[C::OB]) {
+  const KParams& p = t.k;
+  const int n = me & 31, h = (me >> 5) & 1;
+  const int r = q.m * C::ROWS + q.rg * 32 + n;
+  if (r >= t.rows) return;
+  const int node = r / p.heads, head = r - node * p.heads;
+  {
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_sum), __float_as_uint(l_sum), false, false);
+    l_sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    const auto o2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_p), __float_as_uint(l_p), false, false);
+    l_p = __uint_as_float(o2[0]) + __uint_as_float(o2[1]);
+  }
+  if (node >= q.nodes) l_sum = l_p = 0.f;
+  const float inv = empty_sum(l_p) ? 0.f : (q.whole ? ks : 1.f) / l_p;
+  const int col = q.cp * (C::DC / C::NS) + 4 * h;
+  const int64_t row = (int64_t)q.b * p.qrows + node, prow = q.slot * C::ROWS + q.rg * 32 + n;
+  const int64_t orow = q.whole ? row * p.o_sr + head * p.o_sh : prow * C::DC;
+  const int dt = q.whole ? p.out_dt : QMLA_DT_F32;
+  char* ob0 = (q.whole ? reinterpret_cast<char*>(p.out) : reinterpret_cast<char*>(t.part_o)) + (orow + col) * out_bytes(dt);
+  auto store = [&](auto dtc) {
+    constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
+#pragma unroll
+    for (int ob = 0; ob < C::OB; ++ob)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
+        store_out4<DT>(ob0 + (32 * ob + 8 * i4) * ES, v);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
+  else if (dt == QMLA_DT_F16) store(std::integral_constant<int, QMLA_DT_F16>{});
+  else store(std::integral_constant<int, QMLA_DT_BF16>{});
+  if (h == 0 && q.cp == 0) {
+    if (!q.whole) t.part_lse[prow] = empty_sum(l_sum) ? kNegInf : m_ref + fast_log2(l_sum);
+    else if (p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, row_lse(m_ref, l_sum));
+  }
+}
 
 template <class C>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_kernel(const TrParams t) {
@@ -279,6 +406,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 #pragma unroll
     for (int i = 0; i < C::OB; ++i) acc[i] = f32x16{};
     float m_ref = kNegInf, l_sum = 0.f, l_p = 0.f;
+    Soft sf;
 
     // ---- staging
     i32x4 raw[C::LOADS];
@@ -429,34 +557,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
       mfma_v_done(s);
     };
-    // ---- divide, cap, mask
-    auto finish = [&](int j, f32x16& s) {
-      const float* ir = irms + (j % C::STAGES) * p.heads * IRS + irms_at;
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 iv = *reinterpret_cast<const f32x4*>(ir + 8 * i4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
-      }
-      if (p.logit_cap > 0.f) {
-        const float in = 2.0f * kLog2e / p.logit_cap, out = p.logit_cap * kLog2e;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = out - 2.0f * out * __builtin_amdgcn_rcpf(fast_exp2(s[i] * in) + 1.0f);
-      }
-      if ((j + 1) * TT > base) {
-        const uint32_t od = odd[j & 3];
-        const int r = m * C::ROWS + rg * 32 + (own() & 31), node = r / p.heads;
-        const uint64_t sees = r < t.rows && node < nodes ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
-          const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
-          s[i] = !vis ? kNegInf : (od >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
-        }
-      }
-    };
-    // ---- softmax against a reference that moves when a row's maximum has passed it by kMoveAt (a row's own
-    // doing: what its neighbours hold does not move it; a NaN maximum moves nothing)
     auto value_read = [&](uint32_t src, int i) {   // fragment i: columns 32 (i / 2) .., tokens 16 (i % 2) ..
       typedef short i16x8 __attribute__((ext_vector_type(8)));
       i16x4 v[2];
@@ -485,58 +585,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    // the softmax of s in steps 0 .. NSOFT - 1, small enough to lie beside one product each
-    struct Soft {
-      float mx, m_use, m_new, es, ep;
-    } sf;
-    auto soft_step = [&](int i, f32x16& s, bf16x8 (&pn)[2]) {
-      if (i == 0) {
-        sf.mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
-        sf.es = sf.ep = 0.f;
-      } else if (i < 6) {
-        sf.mx = fmaxf(fmaxf(sf.mx, s[2 * i + 1]), s[2 * i + 2]);
-      } else if (i == 6) {
-        sf.mx = fmaxf(fmaxf(sf.mx, s[13]), fmaxf(s[14], s[15]));
-      } else if (i == 7) {
-        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sf.mx), __float_as_uint(sf.mx), false, false);
-        sf.mx = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-        sf.m_new = sf.mx > m_ref + kMoveAt ? sf.mx : m_ref;
-        sf.m_use = is_neg_inf(sf.m_new) ? 0.f : sf.m_new;
-      } else if (i < 16) {
-        const int x = 2 * (i - 8);
-        s[x] = fast_exp2(s[x] - sf.m_use);
-        s[x + 1] = fast_exp2(s[x + 1] - sf.m_use);
-      } else if (i < 24) {
-        const int x = 2 * (i - 16);
-        sf.es += s[x] + s[x + 1];
-        const bf16x2 e{(__bf16)s[x], (__bf16)s[x + 1]};
-        pn[x >> 3][x & 7] = e[0];
-        pn[x >> 3][(x & 7) + 1] = e[1];
-        sf.ep = __builtin_amdgcn_fdot2_f32_bf16(e, bf16x2{(__bf16)1.f, (__bf16)1.f}, sf.ep, false);
-      }
-    };
-    constexpr int NSOFT = 24;
-    auto rescale = [&](float m_new, float es, float ep) {
-      const bool moves = m_new != m_ref;
-      if (__builtin_amdgcn_ballot_w64(moves)) {
-        const float alpha = moves ? fast_exp2(m_ref - m_new) : 1.f;
-        l_sum *= alpha;
-        l_p *= alpha;
-#pragma unroll
-        for (int ob = 0; ob < C::OB; ++ob) {
-          // one block at a time, there and back: left to the compiler all of them pass through VGPRs at
-          // once and displace the queries
-          asm volatile("" : "+a"(acc[ob]));
-          acc[ob] *= alpha;
-          asm volatile("" : "+a"(acc[ob]));
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        m_ref = m_new;
-      }
-      l_sum += es;
-      l_p += ep;
-    };
-
     __syncthreads();   // the last piece's tiles are read
     if (tid < 4) odd[tid] = 0;
     // (rows past the piece's end but inside the request are looked up and not fetched)
@@ -588,7 +636,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         }
       }
       if (wlive) {
-        finish(j, s);
+        finish_scores(t, s, irms + (j % C::STAGES) * p.heads * IRS + irms_at);
+        if ((j + 1) * TT > base) mask_scores(t, s, j, b, base, nodes, m * C::ROWS + rg * 32, own(), odd[j & 3]);
         bf16x8 pn[2];
         if constexpr (PIPE) {
           // (a piece's first step has no tile before it: zeros against its own)
@@ -596,15 +645,15 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           constexpr int PER = 2 * C::OB >= NSOFT ? 1 : 2;   // softmax steps a slot
           values(j > ta ? j - 1 : j, pf, [&](int i) {
 #pragma unroll
-            for (int x = 0; x < PER; ++x) soft_step(PER * i + x, s, pn);
+            for (int x = 0; x < PER; ++x) soft_step(PER * i + x, s, pn, sf, m_ref);
           });
-          rescale(sf.m_new, sf.es, sf.ep);
+          rescale(sf, m_ref, l_sum, l_p, acc);
           pf[0] = pn[0];
           pf[1] = pn[1];
         } else {
 #pragma unroll
-          for (int i = 0; i < NSOFT; ++i) soft_step(i, s, pn);
-          rescale(sf.m_new, sf.es, sf.ep);
+          for (int i = 0; i < NSOFT; ++i) soft_step(i, s, pn, sf, m_ref);
+          rescale(sf, m_ref, l_sum, l_p, acc);
           values(j, pn, [](int) {});
         }
       }
@@ -616,49 +665,417 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     }
     if (PIPE && wlive) values(te - 1, pf, [](int) {});
 
-    // ---- this piece's rows
-    const int me = own(), n = me & 31, h = (me >> 5) & 1;
-    const int r = r0 + n;
-    if (r < t.rows) {
-      const int node = r / p.heads, head = r - node * p.heads;
-      {
-        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_sum), __float_as_uint(l_sum), false, false);
-        l_sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
-        const auto o2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_p), __float_as_uint(l_p), false, false);
-        l_p = __uint_as_float(o2[0]) + __uint_as_float(o2[1]);
-      }
-      if (node >= nodes) l_sum = l_p = 0.f;
-      const bool whole = ta == 0 && te == nt;
-      const int64_t slot = 2 * w + (u > rng.lo ? 1 : 0);
-      const float inv = empty_sum(l_p) ? 0.f : (whole ? ks : 1.f) / l_p;
-      const int col = cp * (C::DC / C::NS) + 4 * h;
-      const int64_t orow = whole ? ((int64_t)b * p.qrows + node) * p.o_sr + head * p.o_sh : (slot * C::ROWS + rg * 32 + n) * C::DC;
-      const int dt = whole ? p.out_dt : QMLA_DT_F32;
-      char* ob0 = (whole ? reinterpret_cast<char*>(p.out) : reinterpret_cast<char*>(t.part_o)) + (orow + col) * out_bytes(dt);
-      auto store = [&](auto dtc) {
-        constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
-#pragma unroll
-        for (int ob = 0; ob < C::OB; ++ob)
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            f32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
-            store_out4<DT>(ob0 + (32 * ob + 8 * i4) * ES, v);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-      };
-      if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
-      else if (dt == QMLA_DT_F16) store(std::integral_constant<int, QMLA_DT_F16>{});
-      else store(std::integral_constant<int, QMLA_DT_BF16>{});
-      if (h == 0 && cp == 0) {
-        if (!whole) t.part_lse[slot * C::ROWS + rg * 32 + n] = empty_sum(l_sum) ? kNegInf : m_ref + fast_log2(l_sum);
-        else if (p.lse) store_out(p.lse, p.lse_dt, ((int64_t)b * p.qrows + node) * p.lse_sr + head, row_lse(m_ref, l_sum));
-      }
-    }
+    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
     u += te - ta;
   }
   report_pages(p, bad);
+}
+
+// ---- FP8 rows as they are --------------------------------------------------------------------------------
+// The tiles stay in LDS as the cache holds them, and a wave converts what it multiplies, beside the products. Staged
+// to bf16 (tree_kernel) they cost each workgroup the conversion before its first product of a step, and the LDS
+// twice the bytes: transposed 16-bit reads run at half the LDS rate, 8-bit ones bring 8 tokens of a column in the
+// same time (B 16 x 64 nodes 533 us staged). The rows arrive by LDS-DMA, A tiles ahead, which holds no registers.
+// Scores on the FP8 products (the query as two e4m3 parts) would need no conversion, but those sum with less than fp32:
+// 1.4e-4 off at scores of 5, 5e-6 of the terms, where the bf16 products give 1e-6.
+template <int DC_, int K_, bool MASKED_, int NS_, int STAGES_, int SR_>
+struct Cfg8 {
+  static constexpr int DC = DC_, NS = NS_, STAGES = STAGES_;
+  static constexpr int SR = SR_;                          // 16-byte chunks of a staged row, odd: 32 rows on distinct banks
+  static constexpr bool MASKED = MASKED_;                 // the last blocks hold other columns than keys
+  static constexpr int ROWS = 128 / NS;
+  static constexpr int NB = 2 * ((DC / 64 + K_ + NS - 1) / NS);   // 32-column score blocks of a wave
+  static constexpr int F0 = DC / 32 - (NS - 1) * NB > 0 ? DC / 32 - (NS - 1) * NB : 0;   // from here on columns may not be keys
+  static constexpr int OB = DC / NS / 32;
+  static constexpr int RSTRIDE = SR * 16, TILE_B = TT * RSTRIDE;
+  static constexpr int CHUNKS = TT * SR, DI = (CHUNKS + NT - 1) / NT;   // DMA instructions of a wave for a tile
+  static constexpr int A = STAGES > 2 ? STAGES - 2 : 1;   // tiles ahead
+  static constexpr bool PIPE = STAGES > 2;
+  static constexpr int IRB = NS == 1 ? 2 : 1;             // tiles of divisors held
+  static constexpr int ROPE_MAX = 64 * K_;
+  static_assert(SR % 2 == 1 && DC % (32 * NS) == 0);
+};
+constexpr int PIDN = 256;   // page ids of a piece held at once
+constexpr int KB = 4, VB = 6;   // score blocks, value fragments read ahead
+
+template <class C>
+__host__ __device__ constexpr int lds_bytes8(int heads) {
+  return C::STAGES * C::TILE_B + C::IRB * heads * IRS * 4 + (C::NS > 1 ? 4 * 4096 : 0) + 8 * TT * 8 + PIDN * 4 + 16;
+}
+
+// 16 bytes a lane from memory to LDS at base + 16 lane, unseen by the compiler, whose waits for its own loads
+// and LDS reads would drain it: counted by wait_vmcnt below
+__device__ __forceinline__ void dma_row(const char* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane((int)base)) : "memory");
+}
+
+template <class C>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree8_kernel(const TrParams t) {
+  extern __shared__ __align__(16) char lds[];
+  typedef __attribute__((address_space(3))) char lchar;
+  const KParams& p = t.k;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int rg = wave / C::NS, cp = wave % C::NS;
+  const uint32_t kt = (uint32_t)(uintptr_t)QMLA_LDS(char, lds);
+  float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [IRB][heads][IRS]
+  char* part = lds + C::STAGES * C::TILE_B + C::IRB * p.heads * IRS * 4; // [4 waves][4][64] 16 bytes
+  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [8][TT]
+  int* pids = reinterpret_cast<int*>(rowoff + 8 * TT);                   // [PIDN]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(pids + PIDN);              // [4], bit per token
+  // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
+  const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  const Range rng = unit_range(t, w, w == 0);
+  if (rng.lo >= rng.hi) return;
+  const float ks = p.k_scale ? *p.k_scale : 1.f;
+  const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
+  const int rows_b = (p.rms_off_b + (t.rms_mode == QMLA_RMS_NONE ? 0 : p.heads * t.rms_b) > t.cols
+                          ? p.rms_off_b + p.heads * t.rms_b : t.cols);   // bytes of a row that are used
+  const bool last_dma = (((C::DI - 1) * 4 + wave) * 64) < C::CHUNKS;    // this wave has its last DMA of a tile
+  auto own = [&]() {
+    int x = tid;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  int64_t u = rng.lo, c0 = rng.c0;
+  int b = rng.b;
+  while (u < rng.hi) {
+    const int nt = tiles_of(t, b);
+    if (u >= c0 + (int64_t)nt * t.rt) {
+      c0 += (int64_t)nt * t.rt;
+      ++b;
+      continue;
+    }
+    const int m = (int)((u - c0) / nt), ta = (int)((u - c0) - (int64_t)m * nt);
+    const int te = rng.hi - u < nt - ta ? ta + (int)(rng.hi - u) : nt;
+    const int L = p.seq_lens[b], nodes = node_count(t, b), base = L - nodes;
+    const int r0 = m * C::ROWS + rg * 32;
+    const bool wlive = r0 < t.rows;
+
+    // ---- staging
+    // page ids [pw, pw + PIDN) of the request in LDS; refilled when a tile's last page lies behind them
+    int pw = page_div(p, ta * TT);
+    const int npg = page_div(p, L - 1) + 1;
+    auto fill_pages = [&]() {
+      const int x = pw + own();
+      if (x < npg) pids[x - pw] = p.bt[b * p.bt_stride + x];
+    };
+    auto rows_of = [&](int j) {   // byte offsets of tile j's rows; rows past the request: the cache's first row
+      const int me = own();
+      if (me < TT) {
+        const int tok = j * TT + me;
+        int64_t off = 0;
+        if (tok < L) {
+          const int pg = page_div(p, tok);
+          int bad = 0;
+          off = checked_page(p, pids[pg - pw], bad) * p.page_stride_b + (int64_t)(tok - pg * p.page_size) * p.token_stride_b;
+          report_pages(p, bad);
+        }
+        rowoff[(j & 7) * TT + me] = off;
+      }
+    };
+    // rows of tile j, with new page ids first where it needs them (the same for all threads)
+    auto rows_refill = [&](int j) {
+      if (j * TT >= L) return;
+      const int last = (j + 1) * TT < L ? (j + 1) * TT - 1 : L - 1;
+      if (page_div(p, last) - pw >= PIDN) {
+        lds_barrier();
+        pw = page_div(p, j * TT);
+        fill_pages();
+        __syncthreads();
+      }
+      rows_of(j);
+    };
+    auto dma = [&](int j, int i) {   // this wave's DMA instruction i of tile j
+      if (i + 1 == C::DI && !last_dma) return;
+      const int id = (i * 4 + wave) * 64 + (own() & 63);
+      const int row = id / C::SR, c = id - row * C::SR;
+      if (C::CHUNKS % 64 == 0 || id < C::CHUNKS) {
+        const char* src = p.kv + rowoff[(j & 7) * TT + row];
+        dma_row(16 * c < rows_b ? src + 16 * c : src, kt + (j % C::STAGES) * C::TILE_B + (i * 4 + wave) * 1024);
+      }
+    };
+    // the DMA of the tiles up to all but the last `left` issued has landed
+    auto wait_left = [&](auto left) {
+      constexpr int N = decltype(left)::value;
+      if (last_dma) wait_vmcnt<N * C::DI>();
+      else wait_vmcnt<N * (C::DI - 1)>();
+    };
+    // tile j's divisors, 8 threads a row; what the drafted tokens hold that is not finite, and rows past the request,
+    // become zeros, the former flagged in `odd`
+    auto divisors = [&](int j) {
+      const int me = own(), row = me >> 3, c = me & 7;
+      const char* src = lds + (j % C::STAGES) * C::TILE_B + row * C::RSTRIDE;
+      float* ir = irms + (j % C::IRB) * p.heads * IRS + row;
+      // unrolled: an inner loop would count as the hottest code, and the queries be spilled around it
+#pragma unroll
+      for (int i = 0; i < MAXH / 8; ++i) {
+        const int hd = c + 8 * i;
+        if (8 * i < p.heads && hd < p.heads) {
+          uint32_t v = 0;
+          if (t.rms_b == 2) {
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(src + p.rms_off_b + 2 * hd);
+            v = at[0] | ((uint32_t)at[1] << 8);
+          } else if (t.rms_mode != QMLA_RMS_NONE) {
+            v = *reinterpret_cast<const uint8_t*>(src + p.rms_off_b + hd);
+          }
+          ir[hd * IRS] = fs * inv_divisor(v, t.rms_mode, ks);
+        }
+      }
+    };
+    auto mend = [&](int j) {
+      const int me = own(), row = me >> 3, tok = j * TT + row;
+      char* src = lds + (j % C::STAGES) * C::TILE_B + row * C::RSTRIDE;
+      if (tok < base) return;
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < (C::DC + C::ROPE_MAX + 127) / 128; ++i) {
+        const int c = (me & 7) + 8 * i;
+        if (16 * c >= t.cols) continue;
+        i32x4 v = *reinterpret_cast<const i32x4*>(src + 16 * c), keys = v;
+        const int left = t.cols - 16 * c;   // columns that are keys
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int bits = 8 * left - 32 * d;
+          const int mask = bits <= 0 ? 0 : bits >= 32 ? -1 : (int)((1u << (bits & 31)) - 1);
+          keys[d] = v[d] & mask;
+          v[d] &= ~mask;
+        }
+        const bool o = any_odd<true>(keys);
+        any = any || o;
+        if (o || tok >= L) *reinterpret_cast<i32x4*>(src + 16 * c) = v;
+      }
+      if (any && tok < L) atomicOr(&odd[j & 3], 1u << row);
+    };
+
+    lds_barrier();   // the last piece's tiles are read
+    if (tid < 4) odd[tid] = 0;
+    fill_pages();
+    __syncthreads();
+#pragma unroll 1
+    for (int x = 0; x <= C::A; ++x) rows_refill(ta + x);
+    lds_barrier();
+#pragma unroll 1
+    for (int x = 0; x < C::A; ++x)
+      if (ta + x < te) {
+#pragma unroll
+        for (int i = 0; i < C::DI; ++i) {
+          dma(ta + x, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+
+    // ---- this lane's query row
+    bf16x8 qf[2 * C::NB];       // products 2 f and 2 f + 1: columns 32 f + 16 h + 0..7 and + 8..15
+    int irms_at;                // this row's head in the divisors
+    {
+      // rows may be aligned to their elements only
+      typedef bf16x8 bf16x8_e __attribute__((aligned(2)));
+      const int r = r0 + n < t.rows ? r0 + n : t.rows - 1, node = r / p.heads, head = r - node * p.heads;
+      irms_at = head * IRS + 4 * h;
+      const int64_t row = (int64_t)b * p.qrows + node;
+      const __bf16* qn = p.q_nope + row * p.qn_sr + head * p.qn_sh;
+      const __bf16* qp = p.q_pe + row * p.qp_sr + head * p.qp_sh;
+      const int whole8 = p.rope_w & ~7;
+      bf16x8 tail{};
+      for (int i = 0; i < (p.rope_w & 7); ++i) {
+        const __bf16 x = qp[whole8 + i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tail[e] = e == i ? x : tail[e];
+      }
+#pragma unroll
+      for (int f = 0; f < 2 * C::NB; ++f) {
+        // dead rows keep what they read: their columns of the products go nowhere
+        const int c = cp * C::NB * 32 + 32 * (f >> 1) + 16 * h + 8 * (f & 1), o = c - C::DC;
+        if (C::NS == 1 && 16 * f < C::DC) {
+          qf[f] = *reinterpret_cast<const bf16x8_e*>(qn + c);
+        } else {
+          bf16x8 v = tail;
+          if (o < 0) v = *reinterpret_cast<const bf16x8_e*>(qn + c);
+          else if (o < whole8) v = *reinterpret_cast<const bf16x8_e*>(qp + o);
+          i32x4 x = __builtin_bit_cast(i32x4, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = o <= whole8 ? x[e] : 0;
+          qf[f] = __builtin_bit_cast(bf16x8, x);
+        }
+      }
+    }
+    f32x16 acc[C::OB];
+#pragma unroll
+    for (int i = 0; i < C::OB; ++i) acc[i] = f32x16{};
+    float m_ref = kNegInf, l_sum = 0.f, l_p = 0.f;
+    Soft sf;
+
+    // ---- scores of tile j, `beside(slot)` in the slots of its 2 NB products; one wave a SIMD: nothing but this
+    // order hides the LDS. A block's keys are converted in the slots of the block before
+    auto score = [&](int j, f32x16& s, auto&& beside) {
+      // 16 bytes of row n from column 32 block + 16 h
+      const int me = own();
+      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + (me & 31) * C::RSTRIDE + ((me & 32) >> 1) + cp * C::NB * 32;
+      typedef __attribute__((address_space(3))) const i32x4 lvec;
+      auto read = [&](int f) { return *(lvec*)(uintptr_t)(src + 32 * f); };
+      auto keys = [&](i32x4 x, int f) {   // bytes past the row's keys go
+        if (C::MASKED && f >= C::F0) {
+          const int left = t.cols - (cp * C::NB + f) * 32 - ((me & 32) >> 1);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const int bits = 8 * left - 32 * d;
+            x[d] = bits <= 0 ? 0 : bits >= 32 ? x[d] : x[d] & (int)((1u << (bits & 31)) - 1);
+          }
+        }
+        return x;
+      };
+      i32x4 k[KB];
+#pragma unroll
+      for (int f = 0; f < KB; ++f) k[f] = read(f);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 lo, hi;
+      fp8x16_to_bf16(keys(k[0], 0), lo, hi);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = 0; f < C::NB; ++f) {
+        if (f + KB < C::NB) k[f % KB] = read(f + KB);
+        if (f == 0) mfma32_v0(s, lo, qf[0]);
+        else mfma32_v(s, lo, qf[2 * f]);
+        i32x4 x{};
+        bf16x8 next;
+        if (f + 1 < C::NB) {
+          x = keys(k[(f + 1) % KB], f + 1);
+          next = fp8x8_to_bf16(i32x2{x[0], x[1]});
+        }
+        beside(2 * f);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma32_v(s, hi, qf[2 * f + 1]);
+        if (f + 1 < C::NB) {
+          lo = next;
+          hi = fp8x8_to_bf16(i32x2{x[2], x[3]});
+        }
+        beside(2 * f + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      mfma_v_done(s);
+    };
+    // values of tile j against P, `beside(i)` in the slot of product i: columns 32 (i / 2) .., tokens 16 (i % 2) ..
+    auto values = [&](int j, const bf16x8 (&pf)[2], auto&& beside) {
+      // 8 bytes of tokens 16 k2 + 4 h + {0..3, 8..11}, columns 32 ob + 16 (lane / 16 % 2) + 8 (lane % 2)
+      const int me = own(), q = (me & 15) >> 1;
+      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + ((q < 4 ? q : q + 4) + ((me & 32) >> 3)) * C::RSTRIDE + (me & 16) +
+                           8 * (me & 1) + cp * (C::DC / C::NS);
+      auto read = [&](int i) {
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)(src + 32 * (i >> 1) + 16 * (i & 1) * C::RSTRIDE));
+      };
+      i32x2 v[VB];
+#pragma unroll
+      for (int i = 0; i < VB; ++i) v[i] = read(i);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 a = fp8x8_to_bf16(v[0]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2 * C::OB; ++i) {
+        acc[i >> 1] = mfma32(a, pf[i & 1], acc[i >> 1]);
+        if (i + VB < 2 * C::OB) v[i % VB] = read(i + VB);
+        if (i + 1 < 2 * C::OB) a = fp8x8_to_bf16(v[(i + 1) % VB]);
+        beside(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // tiles ta and (their divisors a step ahead) ta + 1 are there before step ta
+    if constexpr (C::A > 1 && C::NS == 1) {
+      if (ta + C::A <= te) wait_left(std::integral_constant<int, C::A - 2>{});
+      else wait_vmcnt<0>();
+    } else {
+      if (ta + C::A <= te) wait_left(std::integral_constant<int, C::A - 1>{});
+      else wait_vmcnt<0>();
+    }
+    lds_barrier();
+    if constexpr (C::NS == 1) divisors(ta);
+
+    bf16x8 pf[2] = {};
+    for (int j = ta; j < te; ++j) {
+      lds_barrier();
+      if (tid == 0) odd[(j + 2) & 3] = 0;
+      if constexpr (C::NS > 1) divisors(j);
+      if ((j + 1) * TT > base) {
+        if constexpr (C::NS > 1) lds_barrier();   // the divisors lie in chunks that mend() may write
+        mend(j);
+        lds_barrier();
+      }
+      if (j + C::A + 1 < te) rows_refill(j + C::A + 1);
+      f32x16 s{};
+      const bool more = j + C::A < te;
+      auto stage = [&](int slot) {   // the next tile's DMA, one instruction every other slot
+        if (slot % 2 == 0 && slot / 2 < C::DI && more) dma(j + C::A, slot / 2);
+      };
+      if (wlive) {
+        score(j, s, stage);
+#pragma unroll
+        for (int i = C::NB; i < C::DI; ++i) {
+          if (more) dma(j + C::A, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < C::DI; ++i) {
+          if (more) dma(j + C::A, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if constexpr (C::NS == 1) {
+        if (j + 1 < te) divisors(j + 1);
+      } else {
+        if (wlive) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            *reinterpret_cast<f32x4*>(part + ((wave * 4 + i4) * 64 + lane) * 16) =
+                f32x4{s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]};
+        }
+        lds_barrier();
+        if (wlive) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            f32x4 sum = *reinterpret_cast<const f32x4*>(part + ((rg * C::NS * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int x = 1; x < C::NS; ++x) sum += *reinterpret_cast<const f32x4*>(part + (((rg * C::NS + x) * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * i4 + i] = sum[i];
+          }
+        }
+      }
+      if (wlive) {
+        finish_scores(t, s, irms + (j % C::IRB) * p.heads * IRS + irms_at);
+        if ((j + 1) * TT > base) mask_scores(t, s, j, b, base, nodes, r0, own(), odd[j & 3]);
+        bf16x8 pn[2];
+        if constexpr (C::PIPE) {
+          // (a piece's first step has no tile before it: zeros against its own)
+          constexpr int PER = 2 * C::OB >= NSOFT ? 1 : 2;   // softmax steps a slot
+          static_assert(2 * C::OB * PER >= NSOFT);
+          values(j > ta ? j - 1 : j, pf, [&](int i) {
+#pragma unroll
+            for (int x = 0; x < PER; ++x) soft_step(PER * i + x, s, pn, sf, m_ref);
+          });
+          rescale(sf, m_ref, l_sum, l_p, acc);
+          pf[0] = pn[0];
+          pf[1] = pn[1];
+        } else {
+#pragma unroll
+          for (int i = 0; i < NSOFT; ++i) soft_step(i, s, pn, sf, m_ref);
+          rescale(sf, m_ref, l_sum, l_p, acc);
+          values(j, pn, [](int) {});
+        }
+      }
+      // the next step's tile (and, a step ahead for its divisors, the one behind it) has landed
+      if constexpr (C::A > 1 && C::NS == 1) {
+        if (more) wait_left(std::integral_constant<int, C::A - 2>{});
+        else wait_vmcnt<0>();
+      } else {
+        if (more) wait_left(std::integral_constant<int, C::A - 1>{});
+        else wait_vmcnt<0>();
+      }
+    }
+    if (C::PIPE && wlive) values(te - 1, pf, [](int) {});
+    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
+    u += te - ta;
+  }
 }
 
 // Rows whose tokens several workgroups shared, and rows of requests without tokens. A wave a row.
@@ -720,12 +1137,23 @@ struct Inst {
   const void* fn;
   const void* combine;
   int (*lds)(int heads);
+  int row_b;        // bytes of a cached row a kernel that stages them as they are has room for (0: any)
+  bool exact;       // rope_w == rope_max only
 };
 
 #define QMLA_TR(FP8, DC, CP, NS, ST, QL) \
   {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST, QL>>, \
-   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST, QL>>(heads); }}
+   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST, QL>>(heads); }, 0, false}
+#define QMLA_TR8(DC, K, M, NS, ST, SR) \
+  {true, DC, 64 * K, 128 / NS, (const void*)&tree8_kernel<Cfg8<DC, K, M, NS, ST, SR>>, \
+   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes8<Cfg8<DC, K, M, NS, ST, SR>>(heads); }, 16 * SR, !M}
+// the first that fits: FP8 rows as they are where their divisors leave them room (24 heads of any format), staged
+// to bf16 with more
 static const Inst kInst[] = {
+    QMLA_TR8(512, 1, false, 1, 6, 39), QMLA_TR8(512, 1, true, 1, 6, 39),
+    QMLA_TR8(256, 2, true, 1, 6, 27),  QMLA_TR8(256, 4, true, 1, 6, 35),
+    QMLA_TR8(768, 2, true, 2, 4, 59),  QMLA_TR8(768, 4, true, 2, 4, 67),
+    QMLA_TR8(1792, 4, true, 4, 2, 131),
     QMLA_TR(true, 512, 576, 1, 3, 4),   QMLA_TR(false, 512, 576, 1, 3, 4),
     QMLA_TR(true, 256, 512, 1, 3, 0),   QMLA_TR(false, 256, 512, 1, 3, 0),
     QMLA_TR(true, 768, 1024, 2, 2, 0),  QMLA_TR(false, 768, 1024, 2, 2, 0),
@@ -733,9 +1161,12 @@ static const Inst kInst[] = {
 };
 
 static const Inst* find(const qmla_decode_params* p) {
+  const int div_b = p->rms_mode == QMLA_RMS_BF16 || p->rms_mode == QMLA_RMS_BF16_BYTES ? 2 : 1;
+  const int64_t cols = (int64_t)p->d_c + p->rope_w;
+  const int64_t end = p->rms_mode == QMLA_RMS_NONE ? cols : (int64_t)p->rms_offset + (int64_t)p->heads * div_b;
   for (const Inst& i : kInst)
-    if (i.fp8 == (p->kv_dtype == QMLA_KV_FP8) && i.d_c == p->d_c && p->rope_w <= i.rope_max && p->heads <= MAXH &&
-        i.lds(p->heads) <= LDS_MAX)
+    if (i.fp8 == (p->kv_dtype == QMLA_KV_FP8) && i.d_c == p->d_c && (i.exact ? p->rope_w == i.rope_max : p->rope_w <= i.rope_max) &&
+        p->heads <= MAXH && i.lds(p->heads) <= LDS_MAX && (i.row_b == 0 || (end <= i.row_b && cols <= i.row_b)))
       return &i;
   return nullptr;
 }
@@ -779,7 +1210,9 @@ int qmla_tree_forward(const qmla_decode_params* p0, const int64_t* tree_mask, in
   if (!rows16(&p)) return QMLA_ERR_ALIGN;
   const int eb = p.kv_dtype == QMLA_KV_FP8 ? 1 : 2;
   // the last load of a row may reach past its columns, never past its 16-byte multiple
-  if ((p.page_size > 1 ? p.token_stride : p.page_stride) * eb < ((int64_t)(p.d_c + p.rope_w) * eb + 15) / 16 * 16) return QMLA_ERR_SHAPE;
+  const int64_t div_b = p.rms_mode == QMLA_RMS_NONE ? 0 : p.rms_mode == QMLA_RMS_BF16 || p.rms_mode == QMLA_RMS_BF16_BYTES ? 2 : 1;
+  const int64_t keys_end = (int64_t)(p.d_c + p.rope_w) * eb, div_end = div_b ? (int64_t)p.rms_offset * eb + p.heads * div_b : 0;
+  if ((p.page_size > 1 ? p.token_stride : p.page_stride) * eb < ((keys_end > div_end ? keys_end : div_end) + 15) / 16 * 16) return QMLA_ERR_SHAPE;
   const tr::Inst* in = tr::find(&p);
   if (!in) return QMLA_ERR_NOKERNEL;
   if (p.rows == 0) return QMLA_OK;
