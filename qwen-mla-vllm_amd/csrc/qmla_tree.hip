@@ -28,7 +28,10 @@ namespace tr {
 constexpr int TT = 32, NT = 256;
 constexpr int LDS_MAX = 160 * 1024;
 constexpr int MAXH = 64;
-constexpr float kMoveAt = 8.f;   // log2 units a row's maximum may pass its softmax reference by
+// log2 units a row's maximum may pass its softmax reference by. Moving the reference multiplies all accumulators, 3500
+// cycles of a wave, which one of 32 rows suffices for: at 8 it came every other tile of scores with a deviation of 2
+// (nats). P and the sums are floats, as exact at 2^24 as at 1, and leave the values 2^80.
+constexpr float kMoveAt = 24.f;
 
 struct TrParams {
   KParams k;
@@ -163,6 +166,7 @@ struct Cfg {
   static constexpr int LOADS = (UPR + 7) / 8;      // loads of a thread
   static constexpr int TILE_B = TT * CP * 2;
   static_assert(DC % (32 * NS) == 0 && CP % (16 * NS) == 0 && CP % 64 == 0);
+  static constexpr int out_col(int ob, int i4) { return 32 * ob + 8 * i4; }   // first of accumulators 4 i4 .., h = 0
 };
 
 constexpr int KD = 5, VD = 4;   // LDS reads ahead of a score product, fragments ahead of a value product
@@ -176,6 +180,9 @@ __host__ __device__ constexpr int lds_bytes(int heads) {
 
 typedef __attribute__((address_space(3))) char lchar;
 
+// all loads are there, for the compiler to know
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // ---- what the kernels share: a tile's scores of a lane's row to P, the running sums, a finished piece ------
 // divide by the divisors (ir: this row's, from LDS, scaled) and cap: log2-domain scores
 __device__ __forceinline__ void finish_scores(const TrParams& t, f32x16& s, const float* ir) {
@@ -186,7 +193,7 @@ __device__ __forceinline__ void finish_scores(const TrParams& t, f32x16& s, cons
     for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= iv[i];
   }
   const float cap = t.k.logit_cap;
-  if (cap > 0.f) {
+  if (__builtin_expect(cap > 0.f, 0)) {
     const float in = 2.0f * kLog2e / cap, out = cap * kLog2e;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = out - 2.0f * out * __builtin_amdgcn_rcpf(fast_exp2(s[i] * in) + 1.0f);
@@ -195,13 +202,19 @@ __device__ __forceinline__ void finish_scores(const TrParams& t, f32x16& s, cons
 // a tile with drafted tokens: what the row's node does not see, and tokens with a bad element
 __device__ __forceinline__ void mask_scores(const TrParams& t, f32x16& s, int j, int b, int base, int nodes, int r0, int me,
                                             uint32_t odd) {
-  const int r = r0 + (me & 31), node = r / t.k.heads, h = (me >> 5) & 1;
-  const uint64_t sees = r < t.rows && node < nodes ? (uint64_t)t.mask[b * t.mask_sr + node] : 0;
+  const int r = r0 + (me & 31), node = r / t.k.heads, h = (me >> 5) & 1, d = j * TT - base;   // -TT < d < nodes <= 64
+  uint64_t sees = 0;
+  if (r < t.rows && node < nodes) sees = (uint64_t)t.mask[b * t.mask_sr + node] & (~0ull >> (64 - nodes));
+  // waited for here: left pending on this path, it would be waited for, and every DMA with it, by the tiles that
+  // never come here
+  wait_loads();
+  const uint32_t vis = (d >= 0 ? (uint32_t)(sees >> d) : (uint32_t)(sees << -d) | ((1u << -d) - 1)) >> (4 * h);
+  odd >>= 4 * h;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int x = 8 * (i >> 2) + 4 * h + (i & 3), nd = j * TT + x - base;
-    const bool vis = nd < 0 || (nd < nodes && ((sees >> (nd & 63)) & 1));
-    s[i] = !vis ? kNegInf : (odd >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
+    const int x = 8 * (i >> 2) + (i & 3);
+    const float v = (odd >> x) & 1 ? __uint_as_float(0x7fc00000u) : s[i];
+    s[i] = (vis >> x) & 1 ? v : kNegInf;
   }
 }
 
@@ -238,10 +251,18 @@ __device__ __forceinline__ void soft_step(int i, f32x16& s, bf16x8 (&pn)[2], Sof
     sf.ep = __builtin_amdgcn_fdot2_f32_bf16(e, bf16x2{(__bf16)1.f, (__bf16)1.f}, sf.ep, false);
   }
 }
+// the accumulators of 16 blocks are in AGPRs, all at once: else the compiler may keep one in VGPRs over the loop and
+// copy it there and back each tile
+template <int OB>
+__device__ __forceinline__ void in_agprs(f32x16 (&a)[OB]) {
+  if constexpr (OB == 16)
+    asm volatile("" : "+a"(a[0]), "+a"(a[1]), "+a"(a[2]), "+a"(a[3]), "+a"(a[4]), "+a"(a[5]), "+a"(a[6]), "+a"(a[7]),
+                 "+a"(a[8]), "+a"(a[9]), "+a"(a[10]), "+a"(a[11]), "+a"(a[12]), "+a"(a[13]), "+a"(a[14]), "+a"(a[15]));
+}
 template <int OB>
 __device__ __forceinline__ void rescale(const Soft& sf, float& m_ref, float& l_sum, float& l_p, f32x16 (&acc)[OB]) {
   const bool moves = sf.m_new != m_ref;
-  if (__builtin_amdgcn_ballot_w64(moves)) {
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
     const float alpha = moves ? fast_exp2(m_ref - sf.m_new) : 1.f;
     l_sum *= alpha;
     l_p *= alpha;
@@ -297,7 +318,7 @@ __device__ __forceinline__ void store_piece(const TrParams& t, const Piece& q, i
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
-        store_out4<DT>(ob0 + (32 * ob + 8 * i4) * ES, v);
+        store_out4<DT>(ob0 + C::out_col(ob, i4) * ES, v);
         __builtin_amdgcn_sched_barrier(0);
       }
   };
@@ -485,7 +506,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           }
         }
       }
-      if ((j + 1) * TT > base) {   // rows past the request; drafted tokens: what is not finite goes into `odd`
+      if (__builtin_expect((j + 1) * TT > base, 0)) {   // rows past the request; drafted tokens: what is not finite goes into `odd`
         const int tok = j * TT + row;
         bool any = false;
 #pragma unroll
@@ -637,7 +658,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
       if (wlive) {
         finish_scores(t, s, irms + (j % C::STAGES) * p.heads * IRS + irms_at);
-        if ((j + 1) * TT > base) mask_scores(t, s, j, b, base, nodes, m * C::ROWS + rg * 32, own(), odd[j & 3]);
+        if (__builtin_expect((j + 1) * TT > base, 0)) mask_scores(t, s, j, b, base, nodes, m * C::ROWS + rg * 32, own(), odd[j & 3]);
         bf16x8 pn[2];
         if constexpr (PIPE) {
           // (a piece's first step has no tile before it: zeros against its own)
@@ -675,9 +696,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 // The tiles stay in LDS as the cache holds them, and a wave converts what it multiplies, beside the products. Staged
 // to bf16 (tree_kernel) they cost each workgroup the conversion before its first product of a step, and the LDS
 // twice the bytes: transposed 16-bit reads run at half the LDS rate, 8-bit ones bring 8 tokens of a column in the
-// same time (B 16 x 64 nodes 533 us staged). The rows arrive by LDS-DMA, A tiles ahead, which holds no registers.
+// same time (16 requests of 64 nodes, 2048 .. 8192 tokens: 533 us staged, 323 us so). The rows arrive by LDS-DMA, A tiles ahead, which holds no registers.
 // Scores on the FP8 products (the query as two e4m3 parts) would need no conversion, but those sum with less than fp32:
 // 1.4e-4 off at scores of 5, 5e-6 of the terms, where the bf16 products give 1e-6.
+static_assert(MAXH <= 64);   // divisors: 8 threads a row, 4 heads a thread, twice
 template <int DC_, int K_, bool MASKED_, int NS_, int STAGES_, int SR_>
 struct Cfg8 {
   static constexpr int DC = DC_, NS = NS_, STAGES = STAGES_;
@@ -691,22 +713,47 @@ struct Cfg8 {
   static constexpr int CHUNKS = TT * SR, DI = (CHUNKS + NT - 1) / NT;   // DMA instructions of a wave for a tile
   static constexpr int A = STAGES > 2 ? STAGES - 2 : 1;   // tiles ahead
   static constexpr bool PIPE = STAGES > 2;
-  static constexpr int IRB = NS == 1 ? 2 : 1;             // tiles of divisors held
+  static constexpr int IRB = PIPE ? 2 : 1;                // tiles of divisors held
+  static constexpr int NX = PIPE ? 6 : 2;                 // steps of the work beside the value products
+  static constexpr int PITCH = (2 * NB - 2) / DI;         // score products from one DMA to the next
   static constexpr int ROPE_MAX = 64 * K_;
+  static_assert(PITCH * (DI - 1) + 2 < 2 * NB);
   static_assert(SR % 2 == 1 && DC % (32 * NS) == 0);
+  // Columns of value block ob: 16 from block_col(ob) and 16 that lie block_gap(ob) behind them. The 8 rows that half a
+  // wave reads 16 columns of lie on banks 28 apart (or another odd multiple of 4), 4 of them odd and 4 even
+  // multiples: 16 columns on they would meet their neighbours', 64 on they fill the gaps. (Read side by side
+  // the values of a step took 1830 cycles, 2 banks at a time.)
+  static constexpr int block_gap(int ob) { return ob / 4 * 128 + 128 <= OB * 32 ? 64 : 32; }
+  static constexpr int block_col(int ob) { return block_gap(ob) == 64 ? ob / 4 * 128 + ob % 4 * 16 : ob / 2 * 64 + ob % 2 * 16; }
+  static constexpr int out_col(int ob, int i4) { return block_col(ob) + i4 / 2 * block_gap(ob) + i4 % 2 * 8; }
+  static_assert(OB % 2 == 0);
 };
+#define QMLA_IN __attribute__((always_inline))   // (calls on unlikely paths are not inlined by themselves)
 constexpr int PIDN = 256;   // page ids of a piece held at once
+// f(0) .. f(N - 1) with constants: what is laid out by slots must not wait for the unroller
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
 constexpr int KB = 4, VB = 6;   // score blocks, value fragments read ahead
 
+__host__ __device__ constexpr int heads4(int heads) { return (heads + 3) & ~3; }
 template <class C>
 __host__ __device__ constexpr int lds_bytes8(int heads) {
-  return C::STAGES * C::TILE_B + C::IRB * heads * IRS * 4 + (C::NS > 1 ? 4 * 4096 : 0) + 8 * TT * 8 + PIDN * 4 + 16;
+  return C::STAGES * C::TILE_B + (C::IRB * heads4(heads) + 4) * IRS * 4 + (C::NS > 1 ? 4 * 4096 : 0) + 8 * TT * 8 + PIDN * 4 + 16 + 1024;
 }
 
-// 16 bytes a lane from memory to LDS at base + 16 lane, unseen by the compiler, whose waits for its own loads
-// and LDS reads would drain it: counted by wait_vmcnt below
-__device__ __forceinline__ void dma_row(const char* src, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane((int)base)) : "memory");
+// 16 bytes a lane of `lanes`, or of none where left <= 0, from memory to LDS at base + 16 lane, unseen by the
+// compiler, whose waits for its own loads and LDS reads would drain it: counted by wait_vmcnt below. Called by whole
+// waves; the lanes are masked here, as a branch around the load costs more than it (a taken one about 115 cycles of a
+// lone wave)
+__device__ __forceinline__ void dma_row(const char* src, uint32_t base, uint64_t lanes, int left) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_cmp_gt_i32 %3, 0\n\ts_cselect_b64 exec, %2, 0\n\tglobal_load_lds_dwordx4 %0, off\n\ts_mov_b64 exec, -1"
+               ::"v"(src), "s"(__builtin_amdgcn_readfirstlane((int)base)), "s"(lanes), "s"(__builtin_amdgcn_readfirstlane(left))
+               : "memory", "scc");
 }
 
 template <class C>
@@ -718,11 +765,13 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   const int n = lane & 31, h = lane >> 5;
   const int rg = wave / C::NS, cp = wave % C::NS;
   const uint32_t kt = (uint32_t)(uintptr_t)QMLA_LDS(char, lds);
-  float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [IRB][heads][IRS]
-  char* part = lds + C::STAGES * C::TILE_B + C::IRB * p.heads * IRS * 4; // [4 waves][4][64] 16 bytes
-  int64_t* rowoff = reinterpret_cast<int64_t*>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [8][TT]
+  const int h4 = heads4(p.heads);
+  float* irms = reinterpret_cast<float*>(lds + C::STAGES * C::TILE_B);   // [IRB][h4][IRS], [4][IRS] for heads past the last
+  char* part = lds + C::STAGES * C::TILE_B + (C::IRB * h4 + 4) * IRS * 4; // [4 waves][4][64] 16 bytes
+  const char** rowoff = reinterpret_cast<const char**>(part + (C::NS > 1 ? 4 * 4096 : 0));   // [8][TT] where rows lie
   int* pids = reinterpret_cast<int*>(rowoff + 8 * TT);                   // [PIDN]
   uint32_t* odd = reinterpret_cast<uint32_t*>(pids + PIDN);              // [4], bit per token
+  float* codes = reinterpret_cast<float*>(odd + 4);                      // [256] what a one-byte divisor multiplies by
   // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
   const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
   const Range rng = unit_range(t, w, w == 0);
@@ -731,12 +780,22 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
   const int rows_b = (p.rms_off_b + (t.rms_mode == QMLA_RMS_NONE ? 0 : p.heads * t.rms_b) > t.cols
                           ? p.rms_off_b + p.heads * t.rms_b : t.cols);   // bytes of a row that are used
-  const bool last_dma = (((C::DI - 1) * 4 + wave) * 64) < C::CHUNKS;    // this wave has its last DMA of a tile
-  auto own = [&]() {
+  codes[tid] = fs * inv_divisor(tid, t.rms_mode, ks);
+  const int last_n = C::CHUNKS - ((C::DI - 1) * 4 + wave) * 64;         // lanes of this wave's last DMA of a tile
+  const uint64_t last_lanes = last_n <= 0 ? 0 : last_n >= 64 ? ~0ull : (1ull << last_n) - 1;
+  auto own = [&]() QMLA_IN {
     int x = tid;
     asm volatile("" : "+v"(x));
     return x;
   };
+  // chunk `lane` of this wave's DMA i: its row in the tile, and the chunks before it in the row (what lies behind the
+  // used bytes: the row's first), 8 bits each, two DMAs a register
+  uint32_t place[(C::DI + 1) / 2] = {};
+#pragma unroll
+  for (int i = 0; i < C::DI; ++i) {
+    const int id = (i * 4 + wave) * 64 + lane, row = id / C::SR, c = id - row * C::SR;
+    place[i / 2] |= ((row < TT ? row : TT - 1) << 8 | (16 * c < rows_b ? c : 0)) << (16 * (i & 1));
+  }
   int64_t u = rng.lo, c0 = rng.c0;
   int b = rng.b;
   while (u < rng.hi) {
@@ -753,77 +812,97 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     const bool wlive = r0 < t.rows;
 
     // ---- staging
-    // page ids [pw, pw + PIDN) of the request in LDS; refilled when a tile's last page lies behind them
-    int pw = page_div(p, ta * TT);
+    // page ids [pw, pw + PIDN) of the request in LDS, checked; refilled when a tile's last page lies behind them
+    int pw = 0;
     const int npg = page_div(p, L - 1) + 1;
-    auto fill_pages = [&]() {
+    auto fill_pages = [&]() QMLA_IN {
       const int x = pw + own();
-      if (x < npg) pids[x - pw] = p.bt[b * p.bt_stride + x];
-    };
-    auto rows_of = [&](int j) {   // byte offsets of tile j's rows; rows past the request: the cache's first row
-      const int me = own();
-      if (me < TT) {
-        const int tok = j * TT + me;
-        int64_t off = 0;
-        if (tok < L) {
-          const int pg = page_div(p, tok);
-          int bad = 0;
-          off = checked_page(p, pids[pg - pw], bad) * p.page_stride_b + (int64_t)(tok - pg * p.page_size) * p.token_stride_b;
-          report_pages(p, bad);
-        }
-        rowoff[(j & 7) * TT + me] = off;
+      if (x < npg) {
+        int bad = 0;
+        pids[x - pw] = checked_page(p, p.bt[b * p.bt_stride + x], bad);
+        report_pages(p, bad);
       }
     };
-    // rows of tile j, with new page ids first where it needs them (the same for all threads)
-    auto rows_refill = [&](int j) {
-      if (j * TT >= L) return;
-      const int last = (j + 1) * TT < L ? (j + 1) * TT - 1 : L - 1;
-      if (page_div(p, last) - pw >= PIDN) {
-        lds_barrier();
-        pw = page_div(p, j * TT);
-        fill_pages();
-        __syncthreads();
-      }
-      rows_of(j);
+    int lim = 0;   // tokens whose pages are there
+    auto refill = [&](int j) QMLA_IN {   // new page ids where tile j needs them (the same for all threads)
+      const int last = (j + 1) * TT < L ? (j + 1) * TT : L;
+      if (__builtin_expect(j * TT >= L || last <= lim, 1)) return;
+      lds_barrier();
+      pw = page_div(p, j * TT);
+      const int64_t e = (int64_t)(pw + PIDN) * p.page_size;
+      lim = e < L ? (int)e : L;
+      fill_pages();
+      __syncthreads();
     };
-    auto dma = [&](int j, int i) {   // this wave's DMA instruction i of tile j
-      if (i + 1 == C::DI && !last_dma) return;
-      const int id = (i * 4 + wave) * 64 + (own() & 63);
-      const int row = id / C::SR, c = id - row * C::SR;
-      if (C::CHUNKS % 64 == 0 || id < C::CHUNKS) {
-        const char* src = p.kv + rowoff[(j & 7) * TT + row];
-        dma_row(16 * c < rows_b ? src + 16 * c : src, kt + (j % C::STAGES) * C::TILE_B + (i * 4 + wave) * 1024);
-      }
+    // where tile j's rows lie (rows past the request: its last), 8 threads a row, in two steps
+    auto row_token = [&](int j) {
+      const int tok = j * TT + (own() & 31);
+      return tok < L ? tok : L - 1;
     };
-    // the DMA of the tiles up to all but the last `left` issued has landed
-    auto wait_left = [&](auto left) {
-      constexpr int N = decltype(left)::value;
-      if (last_dma) wait_vmcnt<N * C::DI>();
-      else wait_vmcnt<N * (C::DI - 1)>();
+    auto row_page = [&](int j) { return pids[page_div(p, row_token(j)) - pw]; };
+    auto row_put = [&](int j, int id) {
+      const uint32_t tok = row_token(j), in = tok - page_div(p, tok) * p.page_size;
+      rowoff[(j & 7) * TT + (own() & 31)] = p.kv + ((uint64_t)(uint32_t)id * (uint64_t)p.page_stride_b + (uint64_t)in * (uint32_t)p.token_stride_b);
     };
-    // tile j's divisors, 8 threads a row; what the drafted tokens hold that is not finite, and rows past the request,
-    // become zeros, the former flagged in `odd`
-    auto divisors = [&](int j) {
-      const int me = own(), row = me >> 3, c = me & 7;
-      const char* src = lds + (j % C::STAGES) * C::TILE_B + row * C::RSTRIDE;
-      float* ir = irms + (j % C::IRB) * p.heads * IRS + row;
-      // unrolled: an inner loop would count as the hottest code, and the queries be spilled around it
+    // this wave's DMA instruction i of tile j: where its row lies, itself
+    const char* nx[C::DI];
+    auto placed = [&](int i) {   // (opaque: unpacked ahead of the loop they would take 3 registers a DMA)
+      uint32_t x = place[i / 2];
+      asm volatile("" : "+v"(x));
+      return x >> (16 * (i & 1));
+    };
+    auto dma_row_of = [&](int j, int i) { nx[i] = rowoff[(j & 7) * TT + (placed(i) >> 8 & 255)]; };
+    auto dma = [&](int j, int i) {   // (none from tile te on)
+      dma_row(nx[i] + 16 * (placed(i) & 255), kt + (j % C::STAGES) * C::TILE_B + (i * 4 + wave) * 1024, i + 1 < C::DI ? ~0ull : last_lanes, te - j);
+    };
+    // the DMA of the tiles up to all but the last N issued has landed (DMAs without lanes may not count: waited as if
+    // every wave had one less a tile)
+    auto wait_left = [&](auto left) { wait_vmcnt<decltype(left)::value * (C::DI - (C::CHUNKS % 256 != 0 ? 1 : 0))>(); };
+    // tile j's divisors, 8 threads a row, 4 heads a thread (those of 32 i ..), in two steps
+    typedef __attribute__((address_space(3))) const uint64_t lu64_b __attribute__((aligned(1)));
+    auto div_read = [&](int j, int i) QMLA_IN -> uint64_t {   // (one-byte codes: the lower half)
+      return *(lu64_b*)(uintptr_t)(kt + (j % C::STAGES) * C::TILE_B + (own() >> 3) * C::RSTRIDE + p.rms_off_b +
+                                   ((own() & 7) + 8 * i) * 4 * t.rms_b);
+    };
+    auto div_put = [&](int j, int i, uint64_t v) QMLA_IN {
+      const int hd = 4 * (own() & 7) + 32 * i;
+      float* ir = irms + (hd < h4 ? (j % C::IRB) * h4 + hd : C::IRB * h4) * IRS + (own() >> 3);
+      if (__builtin_expect(t.rms_b == 2, 0)) {
 #pragma unroll
-      for (int i = 0; i < MAXH / 8; ++i) {
-        const int hd = c + 8 * i;
-        if (8 * i < p.heads && hd < p.heads) {
-          uint32_t v = 0;
-          if (t.rms_b == 2) {
-            const uint8_t* at = reinterpret_cast<const uint8_t*>(src + p.rms_off_b + 2 * hd);
-            v = at[0] | ((uint32_t)at[1] << 8);
-          } else if (t.rms_mode != QMLA_RMS_NONE) {
-            v = *reinterpret_cast<const uint8_t*>(src + p.rms_off_b + hd);
-          }
-          ir[hd * IRS] = fs * inv_divisor(v, t.rms_mode, ks);
+        for (int e = 0; e < 4; ++e) {
+          const float r = __uint_as_float((uint32_t)(v >> (16 * e)) << 16);
+          ir[e * IRS] = r > 0.f ? fs * __builtin_amdgcn_rcpf(r) : fs;
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ir[e * IRS] = codes[(uint32_t)v >> (8 * e) & 255];
       }
     };
-    auto mend = [&](int j) {
+    auto divisors = [&](int j) QMLA_IN {
+      div_put(j, 0, div_read(j, 0));
+      if (__builtin_expect(p.heads > 32, 0)) div_put(j, 1, div_read(j, 1));
+    };
+    // the work of step j that lies beside its value products, in steps 0 .. NX - 1: rows of tile j + A + 1, divisors of
+    // tile j + 1
+    int xp = 0;
+    uint64_t xd[2] = {};
+    auto extra = [&](int j, auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i == 0) xp = row_page(j + C::A + 1);
+      else if constexpr (i == 1) row_put(j + C::A + 1, xp);
+      else if constexpr (i == 2) xd[0] = div_read(j + 1, 0);
+      else if constexpr (i == 3) {
+        if (__builtin_expect(p.heads > 32, 0)) xd[1] = div_read(j + 1, 1);
+      } else if constexpr (i == 4) div_put(j + 1, 0, xd[0]);
+      else if (__builtin_expect(p.heads > 32, 0)) div_put(j + 1, 1, xd[1]);
+    };
+    auto extras = [&](int j, auto slot) {
+      constexpr int S = 2 * C::OB, X0 = decltype(slot)::value * C::NX / S, X1 = (decltype(slot)::value + 1) * C::NX / S;
+      each<X1 - X0>([&](auto i) { extra(j, std::integral_constant<int, X0 + decltype(i)::value>{}); });
+    };
+    // what the drafted tokens hold that is not finite, and rows past the request, become zeros, the former flagged
+    // in `odd`
+    auto mend = [&](int j) QMLA_IN {
       const int me = own(), row = me >> 3, tok = j * TT + row;
       char* src = lds + (j % C::STAGES) * C::TILE_B + row * C::RSTRIDE;
       if (tok < base) return;
@@ -850,18 +929,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 
     lds_barrier();   // the last piece's tiles are read
     if (tid < 4) odd[tid] = 0;
-    fill_pages();
-    __syncthreads();
 #pragma unroll 1
-    for (int x = 0; x <= C::A; ++x) rows_refill(ta + x);
+    for (int x = 0; x <= C::A; ++x) {
+      refill(ta + x);
+      row_put(ta + x, row_page(ta + x));
+    }
     lds_barrier();
 #pragma unroll 1
     for (int x = 0; x < C::A; ++x)
       if (ta + x < te) {
 #pragma unroll
         for (int i = 0; i < C::DI; ++i) {
+          dma_row_of(ta + x, i);
           dma(ta + x, i);
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
 
@@ -932,55 +1012,57 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       bf16x8 lo, hi;
       fp8x16_to_bf16(keys(k[0], 0), lo, hi);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int f = 0; f < C::NB; ++f) {
-        if (f + KB < C::NB) k[f % KB] = read(f + KB);
-        if (f == 0) mfma32_v0(s, lo, qf[0]);
+      each<C::NB>([&](auto fc) {
+        constexpr int f = decltype(fc)::value;
+        if constexpr (f + KB < C::NB) k[f % KB] = read(f + KB);
+        if constexpr (f == 0) mfma32_v0(s, lo, qf[0]);
         else mfma32_v(s, lo, qf[2 * f]);
         i32x4 x{};
         bf16x8 next;
-        if (f + 1 < C::NB) {
+        if constexpr (f + 1 < C::NB) {
           x = keys(k[(f + 1) % KB], f + 1);
           next = fp8x8_to_bf16(i32x2{x[0], x[1]});
         }
         beside(2 * f);
         __builtin_amdgcn_sched_barrier(0);
         mfma32_v(s, hi, qf[2 * f + 1]);
-        if (f + 1 < C::NB) {
+        if constexpr (f + 1 < C::NB) {
           lo = next;
           hi = fp8x8_to_bf16(i32x2{x[2], x[3]});
         }
         beside(2 * f + 1);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
       mfma_v_done(s);
     };
     // values of tile j against P, `beside(i)` in the slot of product i: columns 32 (i / 2) .., tokens 16 (i % 2) ..
     auto values = [&](int j, const bf16x8 (&pf)[2], auto&& beside) {
-      // 8 bytes of tokens 16 k2 + 4 h + {0..3, 8..11}, columns 32 ob + 16 (lane / 16 % 2) + 8 (lane % 2)
+      // 8 bytes of tokens 16 k2 + 4 h + {0..3, 8..11}, columns block_col(ob) + block_gap(ob) (lane / 16 % 2) + 8 (lane % 2)
       const int me = own(), q = (me & 15) >> 1;
-      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + ((q < 4 ? q : q + 4) + ((me & 32) >> 3)) * C::RSTRIDE + (me & 16) +
+      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + ((q < 4 ? q : q + 4) + ((me & 32) >> 3)) * C::RSTRIDE +
                            8 * (me & 1) + cp * (C::DC / C::NS);
-      auto read = [&](int i) {
-        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)(src + 32 * (i >> 1) + 16 * (i & 1) * C::RSTRIDE));
+      auto read = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const uint32_t at = src + (me & 16) * (C::block_gap(i >> 1) / 16);
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)(at + C::block_col(i >> 1) + 16 * (i & 1) * C::RSTRIDE));
       };
       i32x2 v[VB];
-#pragma unroll
-      for (int i = 0; i < VB; ++i) v[i] = read(i);
+      each<VB>([&](auto i) { v[i] = read(i); });
       __builtin_amdgcn_sched_barrier(0);
-      bf16x8 a = fp8x8_to_bf16(v[0]);
+      bf16x8 a[2] = {fp8x8_to_bf16(v[0]), fp8x8_to_bf16(v[1])};   // two ahead: a product waits for an operand just written
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 2 * C::OB; ++i) {
-        acc[i >> 1] = mfma32(a, pf[i & 1], acc[i >> 1]);
-        if (i + VB < 2 * C::OB) v[i % VB] = read(i + VB);
-        if (i + 1 < 2 * C::OB) a = fp8x8_to_bf16(v[(i + 1) % VB]);
-        beside(i);
+      in_agprs(acc);
+      each<2 * C::OB>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        acc[i >> 1] = mfma32(a[i & 1], pf[i & 1], acc[i >> 1]);
+        if constexpr (i + VB < 2 * C::OB) v[i % VB] = read(std::integral_constant<int, i + VB>{});
+        if constexpr (i + 2 < 2 * C::OB) a[i & 1] = fp8x8_to_bf16(v[(i + 2) % VB]);
+        beside(ic);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
     };
     // tiles ta and (their divisors a step ahead) ta + 1 are there before step ta
-    if constexpr (C::A > 1 && C::NS == 1) {
+    if constexpr (C::PIPE) {
       if (ta + C::A <= te) wait_left(std::integral_constant<int, C::A - 2>{});
       else wait_vmcnt<0>();
     } else {
@@ -988,70 +1070,39 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       else wait_vmcnt<0>();
     }
     lds_barrier();
-    if constexpr (C::NS == 1) divisors(ta);
+    if constexpr (C::PIPE) divisors(ta);
 
+    wait_loads();   // the queries: as in mask_scores
     bf16x8 pf[2] = {};
     for (int j = ta; j < te; ++j) {
       lds_barrier();
-      if (tid == 0) odd[(j + 2) & 3] = 0;
-      if constexpr (C::NS > 1) divisors(j);
-      if ((j + 1) * TT > base) {
-        if constexpr (C::NS > 1) lds_barrier();   // the divisors lie in chunks that mend() may write
+      in_agprs(acc);
+      odd[(j + 2) & 3] = 0;   // (all threads: a branch costs more)
+      if constexpr (!C::PIPE) divisors(j);
+      if (__builtin_expect((j + 1) * TT > base, 0)) {
+        if constexpr (!C::PIPE) lds_barrier();   // the divisors lie in chunks that mend() may write
         mend(j);
         lds_barrier();
       }
-      if (j + C::A + 1 < te) rows_refill(j + C::A + 1);
+      refill(j + C::A + 1);
       f32x16 s{};
       const bool more = j + C::A < te;
-      auto stage = [&](int slot) {   // the next tile's DMA, one instruction every other slot
-        if (slot % 2 == 0 && slot / 2 < C::DI && more) dma(j + C::A, slot / 2);
+      auto stage = [&](int slot) {   // a tile's DMA, its rows two slots ahead
+        if (slot % C::PITCH == 0 && slot / C::PITCH < C::DI) dma_row_of(j + C::A, slot / C::PITCH);
+        if (slot >= 2 && (slot - 2) % C::PITCH == 0 && (slot - 2) / C::PITCH < C::DI) dma(j + C::A, (slot - 2) / C::PITCH);
       };
-      if (wlive) {
-        score(j, s, stage);
-#pragma unroll
-        for (int i = C::NB; i < C::DI; ++i) {
-          if (more) dma(j + C::A, i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < C::DI; ++i) {
-          if (more) dma(j + C::A, i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      if constexpr (C::NS == 1) {
-        if (j + 1 < te) divisors(j + 1);
-      } else {
-        if (wlive) {
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4)
-            *reinterpret_cast<f32x4*>(part + ((wave * 4 + i4) * 64 + lane) * 16) =
-                f32x4{s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]};
-        }
-        lds_barrier();
-        if (wlive) {
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            f32x4 sum = *reinterpret_cast<const f32x4*>(part + ((rg * C::NS * 4 + i4) * 64 + lane) * 16);
-#pragma unroll
-            for (int x = 1; x < C::NS; ++x) sum += *reinterpret_cast<const f32x4*>(part + (((rg * C::NS + x) * 4 + i4) * 64 + lane) * 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * i4 + i] = sum[i];
-          }
-        }
-      }
-      if (wlive) {
-        finish_scores(t, s, irms + (j % C::IRB) * p.heads * IRS + irms_at);
-        if ((j + 1) * TT > base) mask_scores(t, s, j, b, base, nodes, r0, own(), odd[j & 3]);
+      auto finish = [&]() {   // scores to P, and the values
+        finish_scores(t, s, irms + (j % C::IRB) * h4 * IRS + irms_at);
+        if (__builtin_expect((j + 1) * TT > base, 0)) mask_scores(t, s, j, b, base, nodes, r0, own(), odd[j & 3]);
         bf16x8 pn[2];
         if constexpr (C::PIPE) {
           // (a piece's first step has no tile before it: zeros against its own)
           constexpr int PER = 2 * C::OB >= NSOFT ? 1 : 2;   // softmax steps a slot
           static_assert(2 * C::OB * PER >= NSOFT);
-          values(j > ta ? j - 1 : j, pf, [&](int i) {
+          values(j > ta ? j - 1 : j, pf, [&](auto i) {
 #pragma unroll
             for (int x = 0; x < PER; ++x) soft_step(PER * i + x, s, pn, sf, m_ref);
+            extras(j, i);
           });
           rescale(sf, m_ref, l_sum, l_p, acc);
           pf[0] = pn[0];
@@ -1060,19 +1111,60 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 #pragma unroll
           for (int i = 0; i < NSOFT; ++i) soft_step(i, s, pn, sf, m_ref);
           rescale(sf, m_ref, l_sum, l_p, acc);
-          values(j, pn, [](int) {});
+          values(j, pn, [&](auto i) { extras(j, i); });
+        }
+      };
+      auto idle_dma = [&]() {   // a wave without rows
+#pragma unroll
+        for (int i = 0; i < C::DI; ++i) {
+          dma_row_of(j + C::A, i);
+          dma(j + C::A, i);
+        }
+      };
+      auto idle_work = [&]() { each<C::NX>([&](auto i) { extra(j, i); }); };
+      if constexpr (C::NS == 1) {
+        if (__builtin_expect(wlive, 1)) {
+          score(j, s, stage);
+          finish();
+        } else {
+          idle_dma();
+          idle_work();
+        }
+      } else {
+        if (__builtin_expect(wlive, 1)) {
+          score(j, s, stage);
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            *reinterpret_cast<f32x4*>(part + ((wave * 4 + i4) * 64 + lane) * 16) =
+                f32x4{s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]};
+        } else {
+          idle_dma();
+        }
+        lds_barrier();
+        if (__builtin_expect(wlive, 1)) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            f32x4 sum = *reinterpret_cast<const f32x4*>(part + ((rg * C::NS * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int x = 1; x < C::NS; ++x) sum += *reinterpret_cast<const f32x4*>(part + (((rg * C::NS + x) * 4 + i4) * 64 + lane) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * i4 + i] = sum[i];
+          }
+          finish();
+        } else {
+          idle_work();
         }
       }
       // the next step's tile (and, a step ahead for its divisors, the one behind it) has landed
-      if constexpr (C::A > 1 && C::NS == 1) {
-        if (more) wait_left(std::integral_constant<int, C::A - 2>{});
+      if constexpr (C::PIPE) {
+        if (__builtin_expect(more, 1)) wait_left(std::integral_constant<int, C::A - 2>{});
         else wait_vmcnt<0>();
       } else {
-        if (more) wait_left(std::integral_constant<int, C::A - 1>{});
+        if (__builtin_expect(more, 1)) wait_left(std::integral_constant<int, C::A - 1>{});
         else wait_vmcnt<0>();
       }
     }
-    if (C::PIPE && wlive) values(te - 1, pf, [](int) {});
+    if (C::PIPE && wlive) values(te - 1, pf, [](auto) {});
     store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
     u += te - ta;
   }
@@ -1152,7 +1244,7 @@ struct Inst {
 static const Inst kInst[] = {
     QMLA_TR8(512, 1, false, 1, 6, 39), QMLA_TR8(512, 1, true, 1, 6, 39),
     QMLA_TR8(256, 2, true, 1, 6, 27),  QMLA_TR8(256, 4, true, 1, 6, 35),
-    QMLA_TR8(768, 2, true, 2, 4, 59),  QMLA_TR8(768, 4, true, 2, 4, 67),
+    QMLA_TR8(768, 2, true, 2, 4, 59),  QMLA_TR8(768, 4, true, 2, 4, 65),
     QMLA_TR8(1792, 4, true, 4, 2, 131),
     QMLA_TR(true, 512, 576, 1, 3, 4),   QMLA_TR(false, 512, 576, 1, 3, 4),
     QMLA_TR(true, 256, 512, 1, 3, 0),   QMLA_TR(false, 256, 512, 1, 3, 0),
