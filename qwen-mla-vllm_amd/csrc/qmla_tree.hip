@@ -74,44 +74,70 @@ __device__ __forceinline__ int tiles_of(const TrParams& t, int b) {
   return L <= 0 || node_count(t, b) == 0 ? 0 : (L + TT - 1) / TT;
 }
 
-// Work units are (row tile, token tile) pairs, requests outermost, tokens innermost; workgroup w owns units
-// [w * chunk, (w + 1) * chunk).
+// Work units are (row tile, token tile) pairs, requests outermost, tokens innermost. Either workgroup w owns units
+// [w * chunk, (w + 1) * chunk), which may be the end of one row tile's and the start of the next's, or each row tile's
+// tokens are split evenly over workgroups of their own, at most chunk tiles each. The latter is taken where it
+// needs at most SECOND tiles more a workgroup: a second piece costs its start and its end, about as much as
+// 5 tiles (1 request of 8 nodes, 41 tiles in two row tiles: 43 us with one workgroup on both, 27 us so).
+constexpr int SECOND = 4;
 struct Range {
-  int64_t lo, hi, chunk;
-  int b;
+  int64_t lo, hi;
+  int b, w;
   int64_t c0;   // units before request b
 };
-__device__ inline Range unit_range(const TrParams& t, int w, bool store) {
-  const int lane = threadIdx.x & 63;
+__device__ inline Range unit_range(const TrParams& t) {
+  const int lane = threadIdx.x & 63, blk = blockIdx.x;
+  auto tiles = [&](int base) { return base + lane < t.k.n_req ? tiles_of(t, base + lane) : 0; };
   int64_t total = 0;
-  for (int base = 0; base < t.k.n_req; base += 64) {
-    const int b = base + lane;
-    total += lane_value(wave_incl_sum(b < t.k.n_req ? tiles_of(t, b) : 0), 63);
-  }
-  Range r;
+  for (int base = 0; base < t.k.n_req; base += 64) total += lane_value(wave_incl_sum(tiles(base)), 63);
+  Range r{};
   const int64_t units = total * t.rt;
-  r.chunk = (units + t.nwg - 1) / t.nwg;
-  if (r.chunk < t.min_chunk) r.chunk = t.min_chunk;
-  r.lo = w * r.chunk;
-  r.hi = r.lo + r.chunk < units ? r.lo + r.chunk : units;
-  r.b = 0;
-  r.c0 = 0;
-  if (store && lane == 0) t.plan[0] = r.chunk;
-  if (r.lo >= r.hi && !store) return r;
-  int64_t run = 0;
+  int64_t chunk = (units + t.nwg - 1) / t.nwg;
+  if (chunk < t.min_chunk) chunk = t.min_chunk;
+  int even = 0;   // tiles of a workgroup where none has two row tiles', 0: some have
+  int64_t active = (units + chunk - 1) / chunk;
+  if (chunk < (1 << 24))
+    for (int c = (int)chunk; !even && c <= (int)chunk + SECOND; c += SECOND / 2) {
+      int64_t pieces = 0;
+      for (int base = 0; base < t.k.n_req; base += 64) pieces += lane_value(wave_incl_sum((tiles(base) + c - 1) / c), 63);
+      if (pieces * t.rt <= t.nwg) {
+        even = c;
+        active = pieces * t.rt;
+      }
+    }
+  // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
+  const int per = (int)((active + 7) / 8);
+  r.w = t.nwg % 8 == 0 ? (blk & 7) * per + (blk >> 3) : blk;
+  const bool live = r.w < active && (t.nwg % 8 != 0 || (blk >> 3) < per), store = blk == 0;
+  if (store && lane == 0) t.plan[0] = even ? -even : chunk;
+  if (!live && !store) return r;
+  const int64_t start = even ? r.w : r.w * chunk;
+  int64_t run = 0, before = 0;
+  int nt = 0;
   for (int base = 0; base < t.k.n_req; base += 64) {
-    const int b = base + lane;
-    const int n = b < t.k.n_req ? tiles_of(t, b) : 0;
+    const int b = base + lane, all = tiles(base);
+    const int n = even ? (all + even - 1) / even : all;
     const int in = wave_incl_sum(n);
     const int64_t c = run + in - n;
     if (store && b < t.k.n_req) t.plan[1 + b] = c;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(b < t.k.n_req && c * t.rt <= r.lo);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(b < t.k.n_req && c * t.rt <= start);
     if (m) {
       const int x = 63 - __builtin_clzll(m);
       r.b = base + x;
-      r.c0 = (run + lane_value(in - n, x)) * t.rt;
+      before = (run + lane_value(in - n, x)) * t.rt;
+      nt = lane_value(all, x);
     }
     run += lane_value(in, 63);
+  }
+  if (!live) return r;
+  if (even) {
+    const int k = (nt + even - 1) / even, x = (int)(r.w - before), m = x / k, i = x - m * k;
+    r.lo = (int64_t)m * nt + (int64_t)i * nt / k;
+    r.hi = (int64_t)m * nt + (int64_t)(i + 1) * nt / k;
+  } else {
+    r.lo = start;
+    r.hi = start + chunk < units ? start + chunk : units;
+    r.c0 = before;
   }
   return r;
 }
@@ -306,9 +332,8 @@ __device__ __forceinline__ void store_piece(const TrParams& t, const Piece& q, i
   const float inv = empty_sum(l_p) ? 0.f : (q.whole ? ks : 1.f) / l_p;
   const int col = q.cp * (C::DC / C::NS) + 4 * h;
   const int64_t row = (int64_t)q.b * p.qrows + node, prow = q.slot * C::ROWS + q.rg * 32 + n;
-  const int64_t orow = q.whole ? row * p.o_sr + head * p.o_sh : prow * C::DC;
-  const int dt = q.whole ? p.out_dt : QMLA_DT_F32;
-  char* ob0 = (q.whole ? reinterpret_cast<char*>(p.out) : reinterpret_cast<char*>(t.part_o)) + (orow + col) * out_bytes(dt);
+  const int dt = p.out_dt;
+  char* ob0 = reinterpret_cast<char*>(p.out) + (row * p.o_sr + head * p.o_sh + col) * out_bytes(dt);
   auto store = [&](auto dtc) {
     constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
 #pragma unroll
@@ -322,7 +347,20 @@ __device__ __forceinline__ void store_piece(const TrParams& t, const Piece& q, i
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
+  if (!q.whole) {
+    // as the accumulators lie: [wave][block][accumulators 4 i4 ..][lane] 16 bytes
+    char* at = reinterpret_cast<char*>(t.part_o) + ((q.slot * 4 + q.rg * C::NS + q.cp) * C::OB * 256 + (me & 63)) * 16;
+#pragma unroll
+    for (int ob = 0; ob < C::OB; ++ob)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = empty_sum(l_p) ? 0.f : acc[ob][4 * i4 + i] * inv;
+        *reinterpret_cast<f32x4*>(at + (ob * 4 + i4) * 1024) = v;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  } else if (dt == QMLA_DT_F32) store(std::integral_constant<int, QMLA_DT_F32>{});
   else if (dt == QMLA_DT_F16) store(std::integral_constant<int, QMLA_DT_F16>{});
   else store(std::integral_constant<int, QMLA_DT_BF16>{});
   if (h == 0 && q.cp == 0) {
@@ -344,9 +382,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   char* ql = part + (C::NS > 1 ? 4 * 4096 : 0);                          // [4 waves][QL][64] 16 bytes
   int64_t* rowoff = reinterpret_cast<int64_t*>(ql + 4 * C::QL * 1024);   // [4][TT]
   uint32_t* odd = reinterpret_cast<uint32_t*>(rowoff + 4 * TT);          // [4], bit per token
-  // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
-  const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const Range rng = unit_range(t, w, w == 0);
+  const Range rng = unit_range(t);
   if (rng.lo >= rng.hi) return;
   const float ks = p.k_scale ? *p.k_scale : 1.f;
   const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
@@ -686,7 +722,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     }
     if (PIPE && wlive) values(te - 1, pf, [](int) {});
 
-    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
+    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * rng.w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
     u += te - ta;
   }
   report_pages(p, bad);
@@ -772,9 +808,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   int* pids = reinterpret_cast<int*>(rowoff + 8 * TT);                   // [PIDN]
   uint32_t* odd = reinterpret_cast<uint32_t*>(pids + PIDN);              // [4], bit per token
   float* codes = reinterpret_cast<float*>(odd + 4);                      // [256] what a one-byte divisor multiplies by
-  // consecutive workgroups go to consecutive XCDs: give each XCD consecutive ranges, which share tokens
-  const int w = t.nwg % 8 == 0 ? (blockIdx.x & 7) * (t.nwg >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-  const Range rng = unit_range(t, w, w == 0);
+  const Range rng = unit_range(t);
   if (rng.lo >= rng.hi) return;
   const float ks = p.k_scale ? *p.k_scale : 1.f;
   const float fs = p.sm_scale * ks * (p.logit_cap > 0.f ? 1.f : kLog2e);
@@ -1165,62 +1199,85 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       }
     }
     if (C::PIPE && wlive) values(te - 1, pf, [](auto) {});
-    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
+    store_piece<C>(t, Piece{b, m, nodes, rg, cp, 2 * rng.w + (u > rng.lo ? 1 : 0), ta == 0 && te == nt}, own(), ks, m_ref, l_sum, l_p, acc);
     u += te - ta;
   }
 }
 
-// Rows whose tokens several workgroups shared, and rows of requests without tokens. A wave a row.
-template <int DC, int ROWS>
+// Rows whose tokens several workgroups shared, and rows of requests without tokens. A wave joins one block of 32 rows,
+// as the accumulators lay: whole 1 KB reads, those of 4 shares under way together (a wave a row, share after share:
+// 16 us for 192 rows of 21 shares, 31 us for 1536 rows of 18).
+template <class C>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const TrParams t) {
   const KParams& p = t.k;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int x = blockIdx.x * 4 + wave, m = blockIdx.y, b = blockIdx.z, r = m * ROWS + x;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int v = blockIdx.x * 4 + (threadIdx.x >> 6), wave = v / C::OB, ob = v - wave * C::OB, m = blockIdx.y, b = blockIdx.z;
+  const int rg = wave / C::NS, cp = wave - rg * C::NS, r = m * C::ROWS + rg * 32 + n;
   if (r >= t.rows) return;
   const int node = r / p.heads, head = r - node * p.heads;
   const int64_t row = (int64_t)b * p.qrows + node;
-  const int64_t o = row * p.o_sr + head * p.o_sh;
   const int nt = tiles_of(t, b);
-  if (nt == 0) {
-    for (int c = lane; c < DC; c += 64) store_out(p.out, p.out_dt, o + c, 0.f);
-    if (lane == 0 && p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, kNegInf);
-    return;
-  }
-  const int64_t chunk = t.plan[0], u0 = t.plan[1 + b] * t.rt + (int64_t)m * nt, u1 = u0 + nt;
-  const int w0 = (int)(u0 / chunk), w1 = (int)((u1 - 1) / chunk);
-  if (w0 == w1) return;
-  auto at = [&](int w) {
-    const int64_t start = u0 > w * chunk ? u0 : w * chunk;
-    return ((int64_t)2 * w + (start > w * chunk ? 1 : 0)) * ROWS + x;
-  };
-  float top = kNegInf;
-  for (int w = w0; w <= w1; ++w) top = fmaxf(top, t.part_lse[at(w)]);
-  const float ref = is_neg_inf(top) ? 0.f : top;
-  constexpr int NV = DC / 256;
-  f32x4 acc[NV];
+  f32x16 acc{};
+  float sum = 0.f, top = kNegInf;
+  if (nt > 0) {
+    const int64_t chunk = t.plan[0];
+    int64_t slot;
+    int k, odd;   // shares; the first lies in its workgroup's second slot
+    if (chunk < 0) {
+      k = (nt - (int)chunk - 1) / -(int)chunk;
+      slot = 2 * (t.plan[1 + b] * t.rt + (int64_t)m * k);
+      odd = 0;
+    } else {
+      const int64_t u0 = t.plan[1 + b] * t.rt + (int64_t)m * nt, w0 = u0 / chunk;
+      k = (int)((u0 + nt - 1) / chunk - w0) + 1;
+      slot = 2 * w0;
+      odd = u0 > w0 * chunk ? 1 : 0;
+    }
+    if (k == 1) return;
+    auto at = [&](int i) { return slot + (i < k ? 2 * i + (i == 0 ? odd : 0) : 2 * (k - 1)); };   // (k > 1)
+    const float* lse = t.part_lse + rg * 32 + n;
+    for (int i = 0; i < k; i += 8) {
+      float x[8];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) acc[i] = f32x4{};
-  float sum = 0.f;
-  for (int w = w0; w <= w1; ++w) {
-    const int64_t s = at(w);
-    const float g = fast_exp2(t.part_lse[s] - ref);   // NaN stays NaN
-    sum += g;
-    const float* src = t.part_o + s * DC + 4 * lane;
+      for (int e = 0; e < 8; ++e) x[e] = lse[at(i + e) * C::ROWS];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] += *reinterpret_cast<const f32x4*>(src + 256 * i) * g;
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+    }
+    const float ref = is_neg_inf(top) ? 0.f : top;
+    const f32x4* src = reinterpret_cast<const f32x4*>(t.part_o) + (wave * C::OB + ob) * 256 + lane;
+    for (int i = 0; i < k; i += 4) {
+      float x[4];
+      f32x4 o[4][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = lse[at(i + e) * C::ROWS];
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) o[e][i4] = src[at(i + e) * (4 * C::OB * 256) + i4 * 64];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < k) {
+          const float g = fast_exp2(x[e] - ref);   // NaN stays NaN
+          sum += g;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) acc[c] += o[e][c >> 2][c & 3] * g;
+        }
+    }
   }
   const float ks = p.k_scale ? *p.k_scale : 1.f;
   const float inv = empty_sum(sum) ? 0.f : ks / sum;
-  char* out = reinterpret_cast<char*>(p.out) + (o + 4 * lane) * out_bytes(p.out_dt);
+  const int64_t o0 = row * p.o_sr + head * p.o_sh + cp * (C::DC / C::NS) + 4 * h;
   auto put = [&](auto dtc) {
     constexpr int DT = decltype(dtc)::value, ES = DT == QMLA_DT_F32 ? 4 : 2;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store_out4<DT>(out + 256 * i * ES, acc[i] * inv);
+    for (int i4 = 0; i4 < 4; ++i4)
+      store_out4<DT>(reinterpret_cast<char*>(p.out) + (o0 + C::out_col(ob, i4)) * ES,
+                     f32x4{acc[4 * i4] * inv, acc[4 * i4 + 1] * inv, acc[4 * i4 + 2] * inv, acc[4 * i4 + 3] * inv});
   };
   if (p.out_dt == QMLA_DT_F32) put(std::integral_constant<int, QMLA_DT_F32>{});
   else if (p.out_dt == QMLA_DT_F16) put(std::integral_constant<int, QMLA_DT_F16>{});
   else put(std::integral_constant<int, QMLA_DT_BF16>{});
-  if (lane == 0 && p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, row_lse(top, sum));
+  if (ob == 0 && cp == 0 && h == 0 && p.lse) store_out(p.lse, p.lse_dt, row * p.lse_sr + head, nt > 0 ? row_lse(top, sum) : kNegInf);
 }
 
 struct Inst {
@@ -1228,6 +1285,7 @@ struct Inst {
   int d_c, rope_max, rows;
   const void* fn;
   const void* combine;
+  int combine_wgs;  // of a row tile
   int (*lds)(int heads);
   int row_b;        // bytes of a cached row a kernel that stages them as they are has room for (0: any)
   bool exact;       // rope_w == rope_max only
@@ -1235,10 +1293,10 @@ struct Inst {
 
 #define QMLA_TR(FP8, DC, CP, NS, ST, QL) \
   {FP8, DC, CP - DC, 128 / NS, (const void*)&tree_kernel<Cfg<FP8, DC, CP, NS, ST, QL>>, \
-   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST, QL>>(heads); }, 0, false}
+   (const void*)&tree_combine_kernel<Cfg<FP8, DC, CP, NS, ST, QL>>, DC / NS / 32, [](int heads) { return lds_bytes<Cfg<FP8, DC, CP, NS, ST, QL>>(heads); }, 0, false}
 #define QMLA_TR8(DC, K, M, NS, ST, SR) \
   {true, DC, 64 * K, 128 / NS, (const void*)&tree8_kernel<Cfg8<DC, K, M, NS, ST, SR>>, \
-   (const void*)&tree_combine_kernel<DC, 128 / NS>, [](int heads) { return lds_bytes8<Cfg8<DC, K, M, NS, ST, SR>>(heads); }, 16 * SR, !M}
+   (const void*)&tree_combine_kernel<Cfg8<DC, K, M, NS, ST, SR>>, DC / NS / 32, [](int heads) { return lds_bytes8<Cfg8<DC, K, M, NS, ST, SR>>(heads); }, 16 * SR, !M}
 // the first that fits: FP8 rows as they are where their divisors leave them room (24 heads of any format), staged
 // to bf16 with more
 static const Inst kInst[] = {
@@ -1335,7 +1393,7 @@ int qmla_tree_forward(const qmla_decode_params* p0, const int64_t* tree_mask, in
   if (hipFuncSetAttribute(in->fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return QMLA_ERR_LAUNCH;
   void* args[] = {&t};
   if (hipLaunchKernel(in->fn, dim3(t.nwg), dim3(tr::NT), args, bytes, (hipStream_t)stream) != hipSuccess) return QMLA_ERR_LAUNCH;
-  const hipError_t e = hipLaunchKernel(in->combine, dim3((in->rows + 3) / 4, t.rt, (unsigned)n_req), dim3(256), args, 0, (hipStream_t)stream);
+  const hipError_t e = hipLaunchKernel(in->combine, dim3(in->combine_wgs, t.rt, (unsigned)n_req), dim3(256), args, 0, (hipStream_t)stream);
   return e == hipSuccess ? QMLA_OK : QMLA_ERR_LAUNCH;
 }
 
