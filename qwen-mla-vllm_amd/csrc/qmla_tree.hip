@@ -158,7 +158,7 @@ __device__ __forceinline__ float inv_divisor(uint32_t raw, int mode, float ks) {
   if (mode == QMLA_RMS_LOG8) return fast_exp2(3.0f - (float)raw * (6.0f / 255.0f));
   if (mode == QMLA_RMS_NONE) return 1.f;
   const float r = mode == QMLA_RMS_E4M3 ? fp8_to_f32(raw) * ks : bf16_bits_to_f32(raw);
-  return r > 0.f ? 1.f / r : 1.f;
+  return r > 0.f ? __builtin_amdgcn_rcpf(r) : 1.f;   // within 1 ulp
 }
 
 // any element of 16 bytes not finite
@@ -201,7 +201,7 @@ constexpr int IRS = TT + 4;   // floats of a head's divisors in LDS
 
 template <class C>
 __host__ __device__ constexpr int lds_bytes(int heads) {
-  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 4 * C::QL * 1024 + 4 * TT * 8 + 16;
+  return C::STAGES * (C::TILE_B + heads * IRS * 4) + (C::NS > 1 ? 4 * 4096 : 0) + 4 * C::QL * 1024 + 4 * TT * 8 + 32;
 }
 
 typedef __attribute__((address_space(3))) char lchar;
@@ -511,18 +511,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           if (8 * i < rdw) rraw[i] = *reinterpret_cast<const uint32_t*>(rs + 4 * (c + 8 * i < rdw ? c + 8 * i : 0));
       }
     };
-    auto put_rms = [&](float* o, int d, uint32_t v) {   // dword d of a row's divisors
-      if (t.rms_b == 1) {
+    // dword d of a row's divisors (heads past the last go into `none`: branches around their stores cost more)
+    auto put_rms = [&](float* o, int d, uint32_t v) {
+      float* none = reinterpret_cast<float*>(odd + 4);
+      auto put1 = [&](int hd, float x) { *((uint32_t)hd < (uint32_t)p.heads ? o + hd * IRS : none) = x; };
+      if (__builtin_expect(t.rms_b == 1, C::FP8)) {
         const int hd = 4 * d - rskip;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((uint32_t)(hd + e) < (uint32_t)p.heads) o[(hd + e) * IRS] = fs * inv_divisor((v >> (8 * e)) & 0xff, t.rms_mode, ks);
+        for (int e = 0; e < 4; ++e) put1(hd + e, fs * inv_divisor((v >> (8 * e)) & 0xff, t.rms_mode, ks));
       } else {
         // an odd byte offset splits a divisor over two dwords: those rows have theirs read by bytes below
         const int hd = 2 * d - (rskip >> 1);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if ((uint32_t)(hd + e) < (uint32_t)p.heads) o[(hd + e) * IRS] = fs * inv_divisor((v >> (16 * e)) & 0xffff, t.rms_mode, ks);
+        for (int e = 0; e < 2; ++e) put1(hd + e, fs * inv_divisor((v >> (16 * e)) & 0xffff, QMLA_RMS_BF16, ks));
       }
     };
     auto put = [&](int j) {
@@ -571,9 +572,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         }
       }
       float* ir = irms + (j % C::STAGES) * p.heads * IRS + row;
-      if (t.rms_mode == QMLA_RMS_NONE) {
+      if (__builtin_expect(t.rms_mode == QMLA_RMS_NONE, 0)) {
         for (int hd = sc0; hd < p.heads; hd += 8) ir[hd * IRS] = fs;
-      } else if (t.rms_b == 2 && (rskip & 1)) {
+      } else if (__builtin_expect(t.rms_b == 2 && (rskip & 1), 0)) {
         for (int hd = sc0; hd < p.heads; hd += 8) {
           const int64_t off_put = rowoff[(j & 3) * TT + row];
           const uint8_t* at = reinterpret_cast<const uint8_t*>(p.kv + off_put + p.rms_off_b + 2 * hd);
@@ -582,7 +583,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       } else {
 #pragma unroll
         for (int i = 0; i < RL; ++i)
-          if (sc0 + 8 * i < rdw) put_rms(ir, sc0 + 8 * i, rraw[i]);
+          if (8 * i < rdw) put_rms(ir, sc0 + 8 * i, rraw[i]);
         // many heads: the rest of the divisors without a step's head start
         for (int d = sc0 + 8 * RL; d < rdw; d += 8) {
           const int64_t off_put = rowoff[(j & 3) * TT + row];
@@ -662,7 +663,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     bf16x8 pf[2] = {};
     for (int j = ta; j < te; ++j) {
       __syncthreads();
-      if (tid == 0) odd[(j + 2) & 3] = 0;
+      in_agprs(acc);
+      odd[(j + 2) & 3] = 0;
       if constexpr (C::STAGES > 1) {
         if (j + 1 < te) put(j + 1);
       }
@@ -672,16 +674,16 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         if (j + 2 < te) fetch(j + 2);
       }
       f32x16 s{};
-      if (wlive) score(j, s);
+      if (__builtin_expect(wlive, 1)) score(j, s);
       if constexpr (C::NS > 1) {
-        if (wlive) {
+        if (__builtin_expect(wlive, 1)) {
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4)
             *reinterpret_cast<f32x4*>(part + ((wave * 4 + i4) * 64 + lane) * 16) =
                 f32x4{s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]};
         }
         __syncthreads();
-        if (wlive) {
+        if (__builtin_expect(wlive, 1)) {
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
             f32x4 sum = *reinterpret_cast<const f32x4*>(part + ((rg * C::NS * 4 + i4) * 64 + lane) * 16);
@@ -692,7 +694,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           }
         }
       }
-      if (wlive) {
+      if (__builtin_expect(wlive, 1)) {
         finish_scores(t, s, irms + (j % C::STAGES) * p.heads * IRS + irms_at);
         if (__builtin_expect((j + 1) * TT > base, 0)) mask_scores(t, s, j, b, base, nodes, m * C::ROWS + rg * 32, own(), odd[j & 3]);
         bf16x8 pn[2];
