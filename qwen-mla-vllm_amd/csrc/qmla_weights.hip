@@ -22,6 +22,7 @@ namespace qmla {
 namespace wt {
 
 constexpr int U = 9;             // loads of a group
+constexpr int QB = 7;            // query loads of a lane under way together
 constexpr int MAXRB = 8;         // row blocks of 16 held at once
 constexpr int LDS_MAX = 160 * 1024;
 
@@ -40,8 +41,6 @@ struct WtParams {
   int steps;       // 16-byte loads of a lane for one token, and how many of them hold keys only
   int whole;
   int passes;      // passes over the tokens, NRB row blocks each
-  uint32_t head_mul;   // x / heads
-  int head_sh;
   int rms_mode, rms_b;   // divisor bytes of a head
   int rms4;        // 4 heads' divisors load at once
 };
@@ -49,9 +48,80 @@ struct WtParams {
 // queries may be aligned to their elements only
 typedef bf16x8 bf16x8_e __attribute__((aligned(2)));
 
-__device__ __forceinline__ float divisor(uint32_t raw, int mode, float ks) {
+__device__ __forceinline__ float inv_divisor(uint32_t raw, int mode, float ks) {
   const float r = mode == QMLA_RMS_E4M3 ? fp8_to_f32(raw) * ks : bf16_bits_to_f32(raw);
-  return r > 0.f ? r : 1.f;
+  return r > 0.f ? __builtin_amdgcn_rcpf(r) : 1.f;   // within 1 ulp
+}
+
+// a query row: where it lies, and its head's latent group
+struct RowAt {
+  const __bf16 *qn, *qp;
+};
+// where the 8 columns from c0 of a query row lie
+struct QueryAt {
+  const __bf16* src;
+  int o, q;          // the first column's place in the latent part and in the rotary one
+  bool whole, part;  // all 8 in one of them; some
+};
+__device__ __forceinline__ QueryAt query_at(const WtParams& w, const RowAt& row, int group, int c0) {
+  QueryAt a;
+  a.o = c0 - group * w.dcg;
+  a.q = c0 - w.d_c;
+  const bool live = group >= 0, latent = a.o >= 0 && a.o + 8 <= w.dcg, rope = !latent && a.q >= 0 && a.q + 8 <= w.k.rope_w;
+  a.src = !live ? reinterpret_cast<const __bf16*>(w.k.kv) : latent ? row.qn + a.o : rope ? row.qp + a.q : reinterpret_cast<const __bf16*>(w.k.kv);
+  a.whole = live && (latent || rope);
+  a.part = live && !latent && !rope && a.o + 8 > 0 && c0 < w.cols && (a.o < w.dcg || a.q + 8 > 0);
+  return a;
+}
+
+// A workgroup's tokens, in units of T (its waves' tiles): each request's split evenly over workgroups of their own, if
+// that takes at most one unit more than an even split of all, which it falls back to. With tokens of two requests
+// a workgroup loads and lays out queries twice, as long as one or two units take (9 requests of 96 rows, 500 .. 12000
+// tokens: 35 us, 29 us so).
+template <int T, class F>
+__device__ __forceinline__ void for_each_piece(const KParams& p, F&& f) {
+  const int lane = threadIdx.x & 63;
+  auto units = [&](int b) { return b < p.n_req ? (req_len(p, b) + T - 1) / T : 0; };
+  int64_t total = 0;
+  for (int base = 0; base < p.n_req; base += 64) total += lane_value(wave_incl_sum(units(base + lane)), 63);
+  const int64_t per = (total + p.nwg - 1) / p.nwg;
+  int64_t lo = 0, hi = 0, c0 = 0;   // units [lo, hi), c0 before request b
+  int b = 0;
+  bool found = false;
+  for (int64_t c = per; !found && c > 0 && c <= per + 1 && c < 1 << 24; ++c) {
+    int64_t pieces = 0;
+    lo = hi = 0;
+    for (int base = 0; base < p.n_req; base += 64) {
+      const int n = units(base + lane), k = (n + (int)c - 1) / (int)c, in = wave_incl_sum(k);
+      const int64_t x = (int64_t)blockIdx.x - pieces;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(in - k <= x && x < in);
+      if (m) {
+        const int l = __builtin_ctzll(m), nl = lane_value(n, l), kl = lane_value(k, l), y = (int)(x - lane_value(in - k, l));
+        b = base + l;
+        lo = (int64_t)nl * y / kl;
+        hi = (int64_t)nl * (y + 1) / kl;
+      }
+      pieces += lane_value(in, 63);
+    }
+    found = pieces <= p.nwg;
+  }
+  if (!found) {
+    lo = blockIdx.x * per;
+    hi = lo + per < total ? lo + per : total;
+    b = 0;
+  }
+  while (lo < hi) {
+    const int L = req_len(p, b);
+    const int64_t n = (L + T - 1) / T;
+    if (lo >= c0 + n) {
+      c0 += n;
+      ++b;
+      continue;
+    }
+    const int64_t a = lo - c0, e = hi - c0 < n ? hi - c0 : n;
+    f(b, (int)a * T, e * T < L ? (int)e * T : L, L);
+    lo += e - a;
+  }
 }
 
 // Up to two row blocks (32 rows): three workgroups a CU of four waves; more: their queries take the LDS of one
@@ -69,49 +139,28 @@ __global__ __launch_bounds__(NRB <= 2 ? 256 : 512, NRB <= 2 ? 3 : 2) void weight
   float* lse_s = reinterpret_cast<float*>(lds + NRB * nm * 1024);   // [NRB * 16], log2 domain
   int* lim_s = reinterpret_cast<int*>(lse_s + NRB * 16);            // tokens a row sees
   int* div_s = lim_s + NRB * 16;                                    // byte of a row's divisor in the cached row
+  int* group_s = div_s + NRB * 16;                                  // its head's latent group, -1: no row
+  RowAt* row_s = reinterpret_cast<RowAt*>(group_s + NRB * 16);
   const float ks = p.k_scale ? *p.k_scale : 1.f;
   int bad = 0;
-  for_each_segment<32, 0>(p, [&](int b, int a, int e, int L, const SegOut&) {
+  for_each_piece<16 * NWV>(p, [&](int b, int a, int e, int L) {
     // a request's pages are its last row's, as its length
     const int* bt = p.bt + ((int64_t)b * p.qrows + p.qrows - 1) * p.bt_stride;
     for (int pass = 0; pass < w.passes; ++pass) {
       const int rbase = pass * NRB * 16;
       __syncthreads();
-#pragma unroll 6
-      for (int x = wave; x < NRB * nm; x += NWV) {
-        const int m = x / NRB, rb = x - m * NRB;
-        const int r = rbase + rb * 16 + n;
-        bf16x8 v{};
-        if (r < w.rows) {
-          const int j = (int)magic_div((uint32_t)r, w.head_mul, w.head_sh), hd = r - j * p.heads;
-          const int64_t row = (int64_t)b * p.qrows + j;
-          const int c0 = FP8 ? 64 * (m >> 1) + 16 * lg + 8 * (m & 1) : 32 * m + 8 * lg;
-          const int o = c0 - (p.heads > p.hpg && hd >= p.hpg ? hd / p.hpg * w.dcg : 0), q = c0 - w.d_c;
-          const __bf16* qn = p.q_nope + row * p.qn_sr + hd * p.qn_sh;
-          const __bf16* qp = p.q_pe + row * p.qp_sr + hd * p.qp_sh;
-          if (o >= 0 && o + 8 <= w.dcg) {
-            v = *reinterpret_cast<const bf16x8_e*>(qn + o);
-          } else if (q >= 0 && q + 8 <= p.rope_w) {
-            v = *reinterpret_cast<const bf16x8_e*>(qp + q);
-          } else if (o + 8 > 0 && c0 < w.cols && (o < w.dcg || q + 8 > 0)) {
-            for (int i = 0; i < 8; ++i) {
-              __bf16 y = (__bf16)0.f;
-              if (o + i >= 0 && o + i < w.dcg) y = qn[o + i];
-              else if (q + i >= 0 && q + i < p.rope_w) y = qp[q + i];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) v[k] = k == i ? y : v[k];
-            }
-          }
-        }
-        qf[(rb * nm + m) * 64 + lane] = v;
-      }
       for (int x = threadIdx.x; x < NRB * 16; x += NT) {
         const int r = rbase + x;
         float l = -kNegInf;   // adds nothing
-        int lim = 0, at = p.rms_off_b;
+        int lim = 0, at = p.rms_off_b, group = -1;
+        RowAt row{};
         if (r < w.rows) {
           const int j = r / p.heads, hd = r - j * p.heads;
-          l = w.lse[((int64_t)b * p.qrows + j) * w.lse_sr + hd];
+          const int64_t qrow = (int64_t)b * p.qrows + j;
+          group = p.heads > p.hpg ? hd / p.hpg : 0;
+          row.qn = p.q_nope + qrow * p.qn_sr + hd * p.qn_sh;
+          row.qp = p.q_pe + qrow * p.qp_sr + hd * p.qp_sh;
+          l = w.lse[qrow * w.lse_sr + hd];
           l = is_neg_inf(l) ? -kNegInf : l * kLog2e;
           lim = L - (p.qrows - 1 - j);
           at += hd * w.rms_b;
@@ -119,6 +168,47 @@ __global__ __launch_bounds__(NRB <= 2 ? 256 : 512, NRB <= 2 ? 3 : 2) void weight
         lse_s[x] = l;
         lim_s[x] = lim;
         div_s[x] = at;
+        group_s[x] = group;
+        row_s[x] = row;
+      }
+      __syncthreads();
+      // 8 columns of a row a lane: QB loads under way together, from the cache's first bytes where there is nothing to
+      // load; what straddles an end is put together by elements behind them
+      for (int x0 = wave; x0 < NRB * nm; x0 += QB * NWV) {
+        bf16x8 v[QB];
+        auto at = [&](int x) {
+          const int m = x / NRB, rx = 16 * (x - m * NRB) + n;
+          return query_at(w, row_s[rx], group_s[rx], FP8 ? 64 * (m >> 1) + 16 * lg + 8 * (m & 1) : 32 * m + 8 * lg);
+        };
+        uint32_t whole = 0, part = 0;
+#pragma unroll
+        for (int y = 0; y < QB; ++y) {
+          const QueryAt q = at(x0 + y * NWV < NRB * nm ? x0 + y * NWV : x0);
+          v[y] = *reinterpret_cast<const bf16x8_e*>(q.src);
+          whole |= (uint32_t)q.whole << y;
+          part |= (uint32_t)q.part << y;
+        }
+#pragma unroll
+        for (int y = 0; y < QB; ++y) {
+          const int x = x0 + y * NWV;
+          if (x >= NRB * nm) break;
+          i32x4 bits = __builtin_bit_cast(i32x4, v[y]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) bits[k] = (whole >> y) & 1 ? bits[k] : 0;
+          v[y] = __builtin_bit_cast(bf16x8, bits);
+          if (__builtin_expect((part >> y) & 1, 0)) {
+            const QueryAt q = at(x);
+            const RowAt row = row_s[16 * (x % NRB) + n];
+            for (int i = 0; i < 8; ++i) {
+              __bf16 e = (__bf16)0.f;
+              if (q.o + i >= 0 && q.o + i < w.dcg) e = row.qn[q.o + i];
+              else if (q.q + i >= 0 && q.q + i < p.rope_w) e = row.qp[q.q + i];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[y][k] = k == i ? e : v[y][k];
+            }
+          }
+          qf[((x % NRB) * nm + x / NRB) * 64 + lane] = v[y];
+        }
       }
       __syncthreads();
       // a tile's page ids are loaded a tile ahead, its divisors and its old weights before its keys
@@ -197,50 +287,36 @@ __global__ __launch_bounds__(NRB <= 2 ? 256 : 512, NRB <= 2 ? 3 : 2) void weight
         const bool edge = t0 + 16 > L - (p.qrows - 1);
         const float f = p.sm_scale * ks;
         float sum = 0.f;
+        // inv(r4, rb, i): f over the divisor of row r4 + i; chosen once a tile, a branch a row costs more than the row
+        auto add = [&](auto inv) {
 #pragma unroll
-        for (int rb = 0; rb < NRB; ++rb) {
-          {
-            const int x = rb * 16 + 4 * lg;
-            float inv[4];
-            if (w.rms_mode == QMLA_RMS_NONE) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) inv[i] = f;
-            } else {
-              uint32_t raw[4];
-              if (w.rms4 && w.rms_b == 1) {
-                const uint32_t v = (uint32_t)rraw[rb][0];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[i] = (v >> (8 * i)) & 0xff;
-              } else if (w.rms4) {
-                const i32x2 v = rraw[rb];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[i] = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffff;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint8_t* at = reinterpret_cast<const uint8_t*>(row + div_s[x + i]);
-                  raw[i] = at[0];
-                  if (w.rms_b == 2) raw[i] |= (uint32_t)at[1] << 8;
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                inv[i] = w.rms_mode == QMLA_RMS_LOG8 ? f * fast_exp2(3.0f - (float)raw[i] * (6.0f / 255.0f))
-                                                     : f / divisor(raw[i], w.rms_mode, ks);
-            }
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse_s + x);
-            const i32x4 lim4 = edge ? *reinterpret_cast<const i32x4*>(lim_s + x) : i32x4{};
+          for (int rb = 0; rb < NRB; ++rb) {
+            const int r4 = rb * 16 + 4 * lg;
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse_s + r4);
+            const i32x4 lim4 = *reinterpret_cast<const i32x4*>(lim_s + r4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float v = s[rb][i] * inv[i];
-              if (p.logit_cap > 0.f) v = p.logit_cap * (1.0f - 2.0f / (fast_exp2(2.0f * kLog2e * (v / p.logit_cap)) + 1.0f));
+              float v = s[rb][i] * inv(r4, rb, i);
+              if (__builtin_expect(p.logit_cap > 0.f, 0)) v = p.logit_cap * (1.0f - 2.0f / (fast_exp2(2.0f * kLog2e * (v / p.logit_cap)) + 1.0f));
               const float l = l4[i];
-              bool dead = __float_as_uint(l) == 0x7f800000u;
-              if (edge) dead = dead || t >= lim4[i];
+              const bool dead = __float_as_uint(l) == 0x7f800000u || (edge && t >= lim4[i]);
               const float pr = fast_exp2(v * kLog2e - l);
               sum += dead ? 0.f : pr;
             }
           }
+        };
+        if (w.rms4 && w.rms_mode == QMLA_RMS_LOG8) {
+          add([&](int, int rb, int i) { return f * fast_exp2(3.0f - (float)(((uint32_t)rraw[rb][0] >> (8 * i)) & 0xff) * (6.0f / 255.0f)); });
+        } else if (w.rms4 && w.rms_b == 2) {
+          add([&](int, int rb, int i) { return f * inv_divisor(((uint32_t)rraw[rb][i >> 1] >> (16 * (i & 1))) & 0xffff, QMLA_RMS_BF16, ks); });
+        } else {
+          add([&](int r4, int, int i) {
+            if (w.rms_mode == QMLA_RMS_NONE) return f;
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(row + div_s[r4 + i]);
+            uint32_t raw = at[0];
+            if (w.rms_b == 2) raw |= (uint32_t)at[1] << 8;
+            return w.rms_mode == QMLA_RMS_LOG8 ? f * fast_exp2(3.0f - (float)raw * (6.0f / 255.0f)) : f * inv_divisor(raw, w.rms_mode, ks);
+          });
         }
         sum = sum_lg(sum);
         if (lg == 0 && t < e && t < w.width) *o = before + sum;
@@ -250,7 +326,7 @@ __global__ __launch_bounds__(NRB <= 2 ? 256 : 512, NRB <= 2 ? 3 : 2) void weight
   report_pages(p, bad);
 }
 
-static int lds_bytes(int nrb, int nm) { return nrb * (nm * 1024 + 16 * 3 * 4); }
+static int lds_bytes(int nrb, int nm) { return nrb * (nm * 1024 + 16 * (4 * 4 + 16)); }
 
 template <bool FP8>
 static const void* pick(int nrb) {
@@ -305,7 +381,6 @@ extern "C" int qmla_attention_weights(const qmla_decode_params* p0, const float*
   if (nrb == 5 || nrb == 7) nrb += wt::lds_bytes(nrb + 1, nm) <= wt::LDS_MAX ? 1 : -1;
   const int bytes = wt::lds_bytes(nrb, nm);
   if (bytes > wt::LDS_MAX) return QMLA_ERR_NOKERNEL;
-  page_magic(p.heads, w.head_mul, w.head_sh);
   w.passes = (blocks + nrb - 1) / nrb;
   w.rms_mode = p.rms_mode;
   w.rms_b = p.rms_mode == QMLA_RMS_BF16 || p.rms_mode == QMLA_RMS_BF16_BYTES ? 2 : 1;
