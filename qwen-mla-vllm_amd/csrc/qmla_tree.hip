@@ -1377,6 +1377,7 @@ int qmla_tree_forward(const qmla_decode_params* p0, const int64_t* tree_mask, in
   if ((uintptr_t)p.workspace % 16) return QMLA_ERR_ALIGN;
   tr::TrParams t{};
   t.k = make_kparams(&p);
+  if (p.rms_mode == QMLA_RMS_NONE) t.k.rms_off_b = 0;   // whatever it was: nothing lies there
   t.mask = tree_mask;
   t.mask_sr = mask_stride;
   t.counts = node_counts;

@@ -19,13 +19,29 @@ def _rows32(fn: str, name: str, t: torch.Tensor, dtype, dim: int) -> None:
         raise TypeError(f"{fn}: {name} must be a {dim}-D {dtype} tensor with contiguous rows")
 
 
+def _clash(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Rows of `b` lie on other rows of `a` ([requests, columns], one type): written through one, read through the
+    other, what is read would depend on the order."""
+    if a is b or a.numel() == 0 or b.numel() == 0:
+        return False
+    es, pa, pb = a.element_size(), a.data_ptr(), b.data_ptr()
+    sa, sb, wa, wb = a.stride(0) * es, b.stride(0) * es, a.shape[1] * es, b.shape[1] * es
+    if pa + (a.shape[0] - 1) * sa + wa <= pb or pb + (b.shape[0] - 1) * sb + wb <= pa:
+        return False
+    if a.shape[0] == 1 and b.shape[0] == 1:
+        return pa != pb
+    if sa != sb or sa == 0:
+        return True
+    return pa != pb and not ((pb - pa) % sa >= wa and (pa - pb) % sa >= wb)   # columns of one buffer, beside each other
+
+
 def attention_weights(q_nope, q_rope, kv_cache, block_table, seq_lens, lse, weights, *, d_c=None, rope_w=None,
                       rms_offset=None, page_size, sm_scale, kv_fp8=None, fp8_rms="log8", k_scale=None, qrows=1, groups=1,
                       rms_heads=None, logit_cap=0.0, out=None, status=None):
     """Add to weights [requests, width] (fp32) what every cached token got in a decode step: out[b, t] =
     weights[b, t] + the sum over request b's qrows query rows and heads of exp(score - lse), for t below the
     request's length; later columns stay as they are, tokens from `width` on are left out. Returns `out`, by
-    default `weights` itself.
+    default `weights` itself; no other row of `out` may lie on a row of `weights`.
 
     The other arguments are those of the `forward` call that gave `lse` [rows, H] (fp32), block_table and
     seq_lens flattened one row per query token. Rows that saw no token add nothing. The sum's order is fixed."""
@@ -41,6 +57,8 @@ def attention_weights(q_nope, q_rope, kv_cache, block_table, seq_lens, lse, weig
         raise ValueError(f"attention_weights: weights and out must be [{n_req}, width]")
     if tuple(lse.shape) != (rows, H) or block_table.shape[0] != rows or seq_lens.shape[0] != rows:
         raise ValueError("attention_weights: lse, block_table and seq_lens need one row per query row")
+    if _clash(weights, out):
+        raise ValueError("attention_weights: out must be weights or lie beside it")
     _lib.same_device("attention_weights", "q_nope", q_nope, "q_rope", q_rope, "kv_cache", kv_cache,
                      "block_table", block_table, "seq_lens", seq_lens, "lse", lse, "weights", weights, "out", out,
                      "status", status)
@@ -164,6 +182,8 @@ def _compact_params(p, kv_cache, block_table, index, counts, first, dst_block_ta
         same = weights_out.data_ptr() == weights.data_ptr()
         if dst_block_table is not None and same:
             raise ValueError("cache_compact: weights_out may be weights in place only")
+        if _clash(weights, weights_out):
+            raise ValueError("cache_compact: weights_out must be weights or lie beside it")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise TypeError("cache_compact: status must be an int32 tensor")
     _lib.same_device("cache_compact", "kv_cache", kv_cache, "block_table", block_table, "index", index,

@@ -44,7 +44,7 @@ def tree_forward(q_nope, q_rope, kv_cache, block_table, seq_lens, tree_mask, *, 
     tree_mask [requests, nodes] int64: bit i of word j lets node j see node i (its own bit among them, see
     `tree_mask`); the context before the nodes is seen by all. Rows from n on, and rows that see no token, come
     back as zeros with lse -inf. d_c 256, 512 (rope up to 64), 768 and 1792 (rope up to 256 elsewhere), bf16 and FP8
-    rows with every divisor format, at most 64 heads; other layouts raise NotImplementedError. A non-finite
+    rows with every divisor format, at most 64 heads (53 at d_c 768); other layouts raise NotImplementedError. A non-finite
     element in a drafted token's row makes the rows that see it NaN.
 
     workspace: a `Workspace` (or a uint8 tensor) reserved for `qmla_tree_workspace_bytes`; without one the call

@@ -216,3 +216,42 @@ def test_rotary_tables():
                dict(rot=8, max_pos=4, scaling="llama3", factor=2.0, original_max_pos=100, low_freq_factor=4.0, high_freq_factor=4.0)):
         with pytest.raises(ValueError):
             qmla.rotary_table(**kw)
+
+
+def test_rows_that_lie_on_other_rows_are_refused():
+    """Weights read through one view and written through another that is shifted against it; columns of one buffer
+    beside each other are fine (the next refusal is the device's)."""
+    buf = torch.zeros(8 * 100 + 100)
+    w, lens, q = buf[:800].view(8, 100), torch.zeros(8, dtype=torch.int32), torch.zeros(8, 24, 512, dtype=torch.bfloat16)
+    cache, bt = torch.zeros(4, 64, 608, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.int32)
+    idx = torch.zeros(8, 4, dtype=torch.int32)
+
+    def weigh(a, b):
+        qmla.attention_weights(q, None, cache, bt, lens, torch.zeros(8, 24), a, out=b, page_size=64, sm_scale=1.0)
+
+    def compact(a, b, dst=None):
+        qmla.cache_compact(cache, bt, idx, lens, dst_block_table=dst, weights=a, weights_out=b)
+
+    for shift in (1, 50, 100):
+        for call in (weigh, compact):
+            with pytest.raises(ValueError, match="beside"):
+                call(w, buf[shift:shift + 800].view(8, 100))
+    with pytest.raises(ValueError, match="beside"):
+        weigh(w[:, :60], w[:, 30:90])
+    with pytest.raises(ValueError, match="beside"):
+        compact(w[:, :60], w[:, 59:90], bt)
+    for a, b in ((w, w), (w, w.view(8, 100)), (w[:, :50], w[:, 50:]), (w[:, 50:], w[:, :50]), (w, torch.zeros(8, 100))):
+        for call in (weigh, compact):
+            with pytest.raises(ValueError, match="GPU"):
+                call(a, b)
+
+
+@pytest.mark.parametrize("kv,d_c,rope,heads,fits", [
+    (_lib.KV_BF16, 768, 116, 53, True), (_lib.KV_BF16, 768, 116, 54, False), (_lib.KV_FP8, 768, 232, 53, True),
+    (_lib.KV_BF16, 512, 64, 64, True), (_lib.KV_BF16, 1792, 256, 64, True), (_lib.KV_FP8, 1792, 256, 64, True),
+    (_lib.KV_FP8, 256, 256, 64, True), (_lib.KV_FP8, 512, 64, 65, False), (_lib.KV_FP8, 512, 65, 24, False)])
+def test_tree_layouts_that_fit(kv, d_c, rope, heads, fits):
+    p = _lib.DecodeParams()
+    p.rows, p.qrows, p.heads, p.d_c, p.rope_w, p.rms_offset, p.kv_dtype = 8, 4, heads, d_c, rope, d_c + rope, kv
+    p.rms_mode, p.num_workgroups = (_lib.RMS_LOG8 if kv == _lib.KV_FP8 else _lib.RMS_BF16), 256
+    assert (_lib.lib().qmla_tree_workspace_bytes(p) > 0) == fits
