@@ -28,7 +28,9 @@ struct alignas(sizeof(T) * V) Vec {
 };
 
 // One thread a unit: V pairs (half: V elements of each half; interleaved: V pairs side by side, two
-// vectors), or V copied elements.
+// vectors), or V copied elements. Every element is read and written once, 16 bytes a load, and the table's rows come
+// from the L2: bound by the copy rate (12001 tokens of 28 bf16 heads of 256: 80 us, 4.3 TB/s where a copy has 4.9;
+// 33 tokens 4 us).
 template <class T, int V, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RParams r) {
   const qmla_rotary_params& p = r.p;

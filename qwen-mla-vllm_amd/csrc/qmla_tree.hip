@@ -13,8 +13,12 @@
 // With NS = 1 a wave owns 32 rows whole. Wider latents do not fit one wave's registers (32 rows x d_c fp32
 // and 32 rows of queries): NS waves share 32 rows, each with 1/NS of the score columns and of the output
 // columns, and add their partial scores through LDS in one order, so they hold equal scores.
-// FP8 rows become bf16 on their way into LDS (exact). P is bf16, the sum that normalizes is of the same
-// rounded P, the lse of the unrounded.
+// FP8 rows become bf16 exactly, beside the products (tree8_kernel) or, where their rows are too wide for that, on their
+// way into LDS (tree_kernel, which holds the bf16 rows). P is bf16, the sum that normalizes is of the same rounded P, the lse
+// of the unrounded.
+//
+// Bound by what one wave a SIMD issues: 16 FP8 requests of 64 nodes x 24 heads on 2048 .. 8192 tokens take 336 us, where
+// their 213 Gflop alone need 157; the matrix cores are busy 37 % and the vector units 42 % of it.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -10,7 +10,8 @@
 // left the L1 before their second half was asked for, 64 FP8 requests 96 us. The queries wait in LDS in the order
 // of the products, a 1 KB read a product. FP8 keys become bf16 exactly, so scores are exact products summed in
 // fp32: the query as e4m3 parts (the decode's scores) would be 5e-6 of the terms off, too much for a
-// fp32 result.
+// fp32 result. 64 FP8 requests of 4096 .. 16384 tokens: 83 us, 4.0 TB/s of their 329 MB; few tokens are bound by the
+// queries' way into LDS (9 bf16 requests of 96 rows: 27 us).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
