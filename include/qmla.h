@@ -358,7 +358,7 @@ typedef struct qmla_evict_params {
   const int32_t* seq_lens;        /* select: [requests] */
   int32_t* index;                 /* [requests, keep], row stride index_stride (select writes it) */
   int64_t index_stride;
-  int32_t* counts;                /* [requests] (select writes it) */
+  int32_t* counts;                /* [requests] (select writes it; may be seq_lens) */
   int32_t requests, width, keep, sink, recent;
   /* compact */
   void* cache;                    /* [num_pages, page_size, (1,) row] */

@@ -36,7 +36,7 @@ constexpr int KEYS = 36 * 1024;               // keys LDS holds beside the histo
 // pass that counts per wave and one that writes. Waves take contiguous runs, so ranks among equal keys
 // and output places follow from per-wave counts without a barrier per run. KEPT: the keys stay in LDS after
 // the first pass (a request of up to KEYS tokens), else every pass reads the weights again. Bound by the passes of one
-// workgroup over a request (40 requests of 2000 .. 32768 tokens: 38 us, 49 with equal bins of a wave added up first; 1 of
+// workgroup over a request (40 requests of 2000 .. 32768 tokens: 35 us, 46 with equal bins of a wave added up first; 1 of
 // 4100: 11 us).
 template <bool KEPT>
 __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
@@ -49,6 +49,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const EParams e) {
   int L = p.seq_lens[b];
   L = L < 0 ? 0 : L < p.width ? L : p.width;
   int* index = p.index + b * p.index_stride;
+  __syncthreads();   // counts may be seq_lens: all have read theirs
   if (tid == 0) p.counts[b] = L < p.keep ? L : p.keep;
   if (L <= p.keep) {
     for (int i = tid; i < p.keep; i += NT) index[i] = i < L ? i : -1;
@@ -168,47 +169,43 @@ __device__ __forceinline__ int64_t row_at(const EParams& e, const int* table, in
   return id * p.page_stride + (int64_t)(tok - pg * p.page_size) * p.token_stride;
 }
 
-// Out of place: a thread copies MU units of its request's rows, a workgroup's width apart; blockIdx.y is the
-// request. What it moves is not read again here, so past the caches; one unit a thread, as the rows lie apart and
-// waves hide the loads (40 requests, 522 MB of 1200-byte rows: 143 us, 168 with 4 units).
-constexpr int MU = 1;
+// Out of place: a workgroup copies MR rows of request blockIdx.y, looked up once, MU units a thread under way together.
+// What it moves is not read again here, so past the caches. Bound by the copy rate: 40 requests, 522 MB of 1200-byte rows,
+// 104 us (a thread a unit that looks its row up itself 143 us).
+constexpr int MR = 32, MU = 4;
 template <class V>
 __global__ __launch_bounds__(256) void move_kernel(const EParams e) {
+  __shared__ int64_t from[MR], to[MR];
   const qmla_evict_params& p = e.p;
-  const int b = blockIdx.y;
-  const int n = min(max(p.counts[b], 0), p.keep);
-  const uint32_t u0 = blockIdx.x * (256u * MU) + threadIdx.x;
-  if (u0 - threadIdx.x >= (uint32_t)n * (uint32_t)e.chunks) return;
-  const int first = p.first ? p.first[b] : 0;
-  int bad = 0, i[MU], c[MU], tok[MU];
-  int64_t s[MU], d[MU];
-#pragma unroll
-  for (int q = 0; q < MU; ++q) {
-    const uint32_t u = u0 + 256u * q;
-    i[q] = (int)magic_div(u, e.chunk_mul, e.chunk_sh);
-    c[q] = (int)u - i[q] * e.chunks;
-    tok[q] = i[q] < n ? p.index[b * p.index_stride + i[q]] : -1;
+  const int b = blockIdx.y, i0 = blockIdx.x * MR, tid = threadIdx.x;
+  const int rows = min(min(max(p.counts[b], 0), p.keep) - i0, MR);
+  if (rows <= 0) return;
+  if (tid < rows) {
+    const int tok = p.index[b * p.index_stride + i0 + tid], at = (p.first ? p.first[b] : 0) + i0 + tid;
+    int bad = 0;
+    const int64_t s = row_at(e, p.block_table, p.bt_stride, p.bt_cols, b, tok, bad);
+    to[tid] = row_at(e, p.dst_block_table, p.dst_bt_stride, p.dst_bt_cols, b, at, bad);
+    from[tid] = to[tid] < 0 ? -1 : s;
+    if (p.weights_out && (uint32_t)tok < (uint32_t)p.width && (uint32_t)at < (uint32_t)p.weights_out_width)
+      p.weights_out[b * p.weights_out_stride + at] = p.weights[b * p.weights_stride + tok];
+    if (bad && p.status) *p.status = QMLA_ERR_PAGE;
   }
+  __syncthreads();
+  const uint32_t units = (uint32_t)rows * (uint32_t)e.chunks;
+  for (uint32_t u0 = tid; u0 < units; u0 += 256u * MU) {
+    V v[MU];
+    int64_t d[MU];
 #pragma unroll
-  for (int q = 0; q < MU; ++q) {
-    s[q] = d[q] = -1;
-    if (i[q] < n) {
-      s[q] = row_at(e, p.block_table, p.bt_stride, p.bt_cols, b, tok[q], bad);
-      d[q] = row_at(e, p.dst_block_table, p.dst_bt_stride, p.dst_bt_cols, b, first + i[q], bad);
+    for (int q = 0; q < MU; ++q) {
+      const uint32_t u = u0 + 256u * q, r = u < units ? magic_div(u, e.chunk_mul, e.chunk_sh) : 0, c = u - r * e.chunks;
+      const int64_t s = u < units ? from[r] : -1;
+      d[q] = s < 0 ? -1 : to[r] + (int64_t)c * (int)sizeof(V);
+      if (s >= 0) v[q] = __builtin_nontemporal_load((const V*)((const char*)p.cache + s) + c);
     }
-  }
-  V v[MU];
 #pragma unroll
-  for (int q = 0; q < MU; ++q)
-    if (s[q] >= 0 && d[q] >= 0) v[q] = __builtin_nontemporal_load((const V*)((const char*)p.cache + s[q]) + c[q]);
-#pragma unroll
-  for (int q = 0; q < MU; ++q) {
-    if (s[q] >= 0 && d[q] >= 0) __builtin_nontemporal_store(v[q], (V*)((char*)p.cache + d[q]) + c[q]);
-    const int to = first + i[q];
-    if (i[q] < n && c[q] == 0 && p.weights_out && (uint32_t)tok[q] < (uint32_t)p.width && (uint32_t)to < (uint32_t)p.weights_out_width)
-      p.weights_out[b * p.weights_out_stride + to] = p.weights[b * p.weights_stride + tok[q]];
+    for (int q = 0; q < MU; ++q)
+      if (d[q] >= 0) __builtin_nontemporal_store(v[q], (V*)((char*)p.cache + d[q]));
   }
-  if (bad && p.status) *p.status = QMLA_ERR_PAGE;
 }
 
 // In place: one workgroup owns CW units of every row of a request (blockIdx.x names them; the last
@@ -318,12 +315,12 @@ int qmla_cache_compact(const qmla_evict_params* p, void* stream) {
   page_magic(p->page_size, e.page_mul, e.page_sh);
   page_magic(e.chunks, e.chunk_mul, e.chunk_sh);
   const bool in_place = !p->dst_block_table;
-  if ((int64_t)p->keep * e.chunks > 0x7fffffff - 256 * ev::MU) return QMLA_ERR_SHAPE;
+  if ((int64_t)p->keep * e.chunks > 0x7fffffff - 256) return QMLA_ERR_SHAPE;
   const void* fn = v == 16  ? (in_place ? (const void*)&ev::move_in_place_kernel<i32x4> : (const void*)&ev::move_kernel<i32x4>)
                    : v == 4 ? (in_place ? (const void*)&ev::move_in_place_kernel<int> : (const void*)&ev::move_kernel<int>)
                    : v == 2 ? (in_place ? (const void*)&ev::move_in_place_kernel<short> : (const void*)&ev::move_kernel<short>)
                             : (in_place ? (const void*)&ev::move_in_place_kernel<char> : (const void*)&ev::move_kernel<char>);
-  const uint32_t gx = in_place ? (e.chunks + ev::CW - 1) / ev::CW + 1 : ((int64_t)p->keep * e.chunks + 256 * ev::MU - 1) / (256 * ev::MU);
+  const uint32_t gx = in_place ? (e.chunks + ev::CW - 1) / ev::CW + 1 : (p->keep + ev::MR - 1) / ev::MR;
   void* args[] = {&e};
   const hipError_t r = hipLaunchKernel(fn, dim3(gx, p->requests), dim3(in_place ? ev::NT : 256), args, 0, (hipStream_t)stream);
   return r == hipSuccess ? QMLA_OK : QMLA_ERR_LAUNCH;

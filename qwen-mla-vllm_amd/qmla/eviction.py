@@ -131,7 +131,8 @@ def evict_select(weights, seq_lens, keep: int, *, sink: int = 0, recent: int = 0
 
     A request of at most `keep` tokens keeps them all; a longer one its first `sink`, its last `recent` and
     the heaviest of the others by weights [requests, width] (fp32), ties to the lower token, NaN as -inf.
-    index[b, :counts[b]] ascends, the rest of the row is -1. Lengths above `width` count as width."""
+    index[b, :counts[b]] ascends, the rest of the row is -1. Lengths above `width` count as width. counts may be
+    seq_lens itself."""
     p, index, counts = _select_params(weights, seq_lens, keep, sink, recent, index, counts)
     _lib.check("qmla_evict_select", _lib.lib().qmla_evict_select(ctypes.byref(p), _lib.stream()))
     return index, counts
@@ -211,7 +212,8 @@ def evict(kv_cache, block_table, seq_lens, weights, keep: int, *, sink: int = 0,
           weights_out=None, index=None, counts=None, status=None):
     """`evict_select` and `cache_compact` in one call: cut every request to at most `keep` tokens. Returns
     (index, counts); counts are the new lengths. Without dst_block_table rows and weights move in place; with
-    it the rows go to those pages and the weights to weights_out, when given."""
+    it the rows go to those pages and the weights to weights_out, when given. Columns of the weights from the new length on
+    keep what they held: clear them before later tokens add theirs."""
     if dst_block_table is None and weights_out is None:
         weights_out = weights
     p, index, counts = _select_params(weights, seq_lens, keep, sink, recent, index, counts)

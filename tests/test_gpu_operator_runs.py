@@ -85,6 +85,19 @@ def test_tree_two_streams_at_once(gpu, kv, rms):
         assert torch.equal(o, calls[i % 2][4][0]) and torch.equal(lse, calls[i % 2][4][1])
 
 
+def test_select_counts_in_place_of_lengths(gpu):
+    """counts given as the lengths themselves: what a call with its own gives."""
+    import qmla
+    g = torch.Generator().manual_seed(3)
+    w = torch.rand(300, 2500, generator=g).to(gpu)
+    lens = torch.randint(0, 2600, (300,), generator=g).to(torch.int32).to(gpu)
+    want, counts = qmla.evict_select(w, lens, 700, sink=3, recent=100)
+    for _ in range(5):
+        own = lens.clone()
+        got, n = qmla.evict_select(w, own, 700, sink=3, recent=100, counts=own)
+        assert n is own and torch.equal(n, counts) and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("layout,lens", [
     (("bf16", "bf16", 64, 18, 3, 1, 1, 64), [70 + i % 9 for i in range(900)]),   # more requests than workgroups
     (("fp8", "log8", 256, 64, 12, 2, 1, 32), [20000, 1, 64, 0, 65]),             # one that takes nearly all of them
