@@ -19,6 +19,12 @@ def _rows32(fn: str, name: str, t: torch.Tensor, dtype, dim: int) -> None:
         raise TypeError(f"{fn}: {name} must be a {dim}-D {dtype} tensor with contiguous rows")
 
 
+def _written(fn: str, name: str, t: torch.Tensor) -> None:
+    """Rows that are written may not lie on one another."""
+    if t.shape[0] > 1 and t.stride(0) < (t.shape[1] if t.dim() == 2 else 1):
+        raise ValueError(f"{fn}: rows of {name} lie on one another")
+
+
 def _clash(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Rows of `b` lie on other rows of `a` ([requests, columns], one type): written through one, read through the
     other, what is read would depend on the order."""
@@ -57,6 +63,7 @@ def attention_weights(q_nope, q_rope, kv_cache, block_table, seq_lens, lse, weig
         raise ValueError(f"attention_weights: weights and out must be [{n_req}, width]")
     if tuple(lse.shape) != (rows, H) or block_table.shape[0] != rows or seq_lens.shape[0] != rows:
         raise ValueError("attention_weights: lse, block_table and seq_lens need one row per query row")
+    _written("attention_weights", "out", out)
     if _clash(weights, out):
         raise ValueError("attention_weights: out must be weights or lie beside it")
     _lib.same_device("attention_weights", "q_nope", q_nope, "q_rope", q_rope, "kv_cache", kv_cache,
@@ -109,10 +116,12 @@ def _select_params(weights, seq_lens, keep, sink, recent, index, counts):
         _rows32("evict_select", "index", index, torch.int32, 2)
         if tuple(index.shape) != (n, keep):
             raise ValueError(f"evict_select: index must be [{n}, {keep}]")
+        _written("evict_select", "index", index)
     if counts is not None:
         _rows32("evict_select", "counts", counts, torch.int32, 1)
         if counts.shape[0] != n:
             raise ValueError(f"evict_select: counts must be [{n}]")
+        _written("evict_select", "counts", counts)
     _lib.same_device("evict_select", "weights", weights, "seq_lens", seq_lens, "index", index, "counts", counts)
     if index is None:
         index = torch.empty(n, keep, dtype=torch.int32, device=weights.device)
@@ -183,6 +192,7 @@ def _compact_params(p, kv_cache, block_table, index, counts, first, dst_block_ta
         same = weights_out.data_ptr() == weights.data_ptr()
         if dst_block_table is not None and same:
             raise ValueError("cache_compact: weights_out may be weights in place only")
+        _written("cache_compact", "weights_out", weights_out)
         if _clash(weights, weights_out):
             raise ValueError("cache_compact: weights_out must be weights or lie beside it")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):

@@ -84,6 +84,11 @@ def _check_out(name: str, x: torch.Tensor, out: torch.Tensor) -> None:
         raise ValueError(f"rotary: {name}_out must have {name}'s shape and dtype")
     if out.numel() and out.stride(-1) != 1:
         raise ValueError(f"rotary: {name}_out's last dimension must be contiguous")
+    extent = 1
+    for st, size in sorted((st, size) for st, size in zip(out.stride(), out.shape) if size > 1):
+        if st < extent:
+            raise ValueError(f"rotary: elements of {name}_out lie on one another")
+        extent += (size - 1) * st
     if out.numel() == 0 or (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
         return
     (a0, a1), (b0, b1) = _span(x), _span(out)
@@ -121,12 +126,13 @@ def rotary(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, cos
         raise TypeError("rotary: q and k must share dtype and head dim")
     if k is None and k_out is not None:
         raise ValueError("rotary: k_out without k")
+    for name, t, t_out in (("q", q, q_out), ("k", k, k_out)):
+        if t_out is not None:
+            _check_out(name, t, t_out)
     _lib.same_device("rotary", "positions", positions, "q", q, "k", k, "cos_sin", cos_sin, "q_out", q_out,
                      "k_out", k_out)
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_out("q", q, q_out)
     keep = ()
     if positions.dtype != torch.int64:
         positions = positions.to(torch.int64)
@@ -137,8 +143,6 @@ def rotary(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, cos
     if k is not None:
         if k_out is None:
             k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        else:
-            _check_out("k", k, k_out)
         p.k, (p.k_token_stride, p.k_head_stride, _) = k.data_ptr(), k.stride()
         p.k_out, (p.k_out_token_stride, p.k_out_head_stride, _) = k_out.data_ptr(), k_out.stride()
         p.k_heads = k.shape[1]

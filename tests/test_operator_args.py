@@ -255,3 +255,31 @@ def test_tree_layouts_that_fit(kv, d_c, rope, heads, fits):
     p.rows, p.qrows, p.heads, p.d_c, p.rope_w, p.rms_offset, p.kv_dtype = 8, 4, heads, d_c, rope, d_c + rope, kv
     p.rms_mode, p.num_workgroups = (_lib.RMS_LOG8 if kv == _lib.KV_FP8 else _lib.RMS_BF16), 256
     assert (_lib.lib().qmla_tree_workspace_bytes(p) > 0) == fits
+
+
+def test_outputs_that_lie_on_themselves_are_refused():
+    q = torch.zeros(4, 3, 64)
+    pos, table = torch.zeros(4, dtype=torch.int64), qmla.rotary_table(64, 8)
+    flat = torch.zeros(4 * 3 * 64)
+    for out in (torch.zeros(4, 1, 64).expand(4, 3, 64), torch.zeros(1, 3, 64).expand(4, 3, 64),
+                torch.as_strided(flat, (4, 3, 64), (64, 64, 1)), torch.as_strided(flat, (4, 3, 64), (100, 32, 1))):
+        with pytest.raises(ValueError, match="lie on one another"):
+            qmla.rotary(pos, q, None, table, q_out=out)
+    e = torch.zeros(4, 1, 64).expand(4, 3, 64)
+    with pytest.raises(ValueError, match="lie on one another"):
+        qmla.rotary(pos, e, None, table, q_out=e)                      # in place on broadcast heads
+    for out in (q, torch.zeros(3, 4, 64).transpose(0, 1), torch.zeros(4, 5, 80)[:, 1:4, 8:72], torch.zeros(8, 3, 64)[::2]):
+        with pytest.raises(ValueError, match="GPU"):
+            qmla.rotary(pos, q, None, table, q_out=out)
+    w, lens = torch.zeros(8, 100), torch.zeros(8, dtype=torch.int32)
+    one = torch.zeros(1, 100).expand(8, 100)
+    with pytest.raises(ValueError, match="lie on one another"):
+        qmla.evict_select(w, lens, 10, index=torch.zeros(1, 10, dtype=torch.int32).expand(8, 10))
+    with pytest.raises((ValueError, TypeError)):
+        qmla.evict_select(w, lens, 10, counts=torch.zeros(1, dtype=torch.int32).expand(8))
+    cache, bt = torch.zeros(4, 64, 608, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="lie on one another"):
+        qmla.cache_compact(cache, bt, torch.zeros(8, 4, dtype=torch.int32), lens, dst_block_table=bt, weights=w, weights_out=one)
+    with pytest.raises(ValueError, match="lie on one another"):
+        qmla.attention_weights(torch.zeros(8, 24, 512, dtype=torch.bfloat16), None, cache, bt, lens, torch.zeros(8, 24), w, out=one,
+                               page_size=64, sm_scale=1.0)
