@@ -761,14 +761,7 @@ struct Cfg8 {
   static constexpr int ROPE_MAX = 64 * K_;
   static_assert(PITCH * (DI - 1) + 2 < 2 * NB);
   static_assert(SR % 2 == 1 && DC % (32 * NS) == 0);
-  // Columns of value block ob: 16 from block_col(ob) and 16 that lie block_gap(ob) behind them. The 8 rows that half a
-  // wave reads 16 columns of lie on banks 28 apart (or another odd multiple of 4), 4 of them odd and 4 even
-  // multiples: 16 columns on they would meet their neighbours', 64 on they fill the gaps. (Read side by side
-  // the values of a step took 1830 cycles, 2 banks at a time.)
-  static constexpr int block_gap(int ob) { return ob / 4 * 128 + 128 <= OB * 32 ? 64 : 32; }
-  static constexpr int block_col(int ob) { return block_gap(ob) == 64 ? ob / 4 * 128 + ob % 4 * 16 : ob / 2 * 64 + ob % 2 * 16; }
-  static constexpr int out_col(int ob, int i4) { return block_col(ob) + i4 / 2 * block_gap(ob) + i4 % 2 * 8; }
-  static_assert(OB % 2 == 0);
+  static constexpr int out_col(int ob, int i4) { return 32 * ob + 8 * i4; }
 };
 #define QMLA_IN __attribute__((always_inline))   // (calls on unlikely paths are not inlined by themselves)
 constexpr int PIDN = 256;   // page ids of a piece held at once
@@ -1077,17 +1070,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     };
     // values of tile j against P, `beside(i)` in the slot of product i: columns 32 (i / 2) .., tokens 16 (i % 2) ..
     auto values = [&](int j, const bf16x8 (&pf)[2], auto&& beside) {
-      // 8 bytes of tokens 16 k2 + 4 h + {0..3, 8..11}, columns block_col(ob) + block_gap(ob) (lane / 16 % 2) + 8 (lane % 2)
+      // 8 bytes of tokens 16 k2 + 4 h + {0..3, 8..11}, columns 32 ob + 16 (lane / 16 % 2) + 8 (lane % 2). (Some of these
+      // reads meet on banks; columns 64 apart meet on a third as many, in the same time.)
       const int me = own(), q = (me & 15) >> 1;
-      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + ((q < 4 ? q : q + 4) + ((me & 32) >> 3)) * C::RSTRIDE +
+      const uint32_t src = kt + (j % C::STAGES) * C::TILE_B + ((q < 4 ? q : q + 4) + ((me & 32) >> 3)) * C::RSTRIDE + (me & 16) +
                            8 * (me & 1) + cp * (C::DC / C::NS);
-      auto read = [&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const uint32_t at = src + (me & 16) * (C::block_gap(i >> 1) / 16);
-        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)(at + C::block_col(i >> 1) + 16 * (i & 1) * C::RSTRIDE));
+      auto read = [&](int i) {
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)(src + 32 * (i >> 1) + 16 * (i & 1) * C::RSTRIDE));
       };
       i32x2 v[VB];
-      each<VB>([&](auto i) { v[i] = read(i); });
+#pragma unroll
+      for (int i = 0; i < VB; ++i) v[i] = read(i);
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 a[2] = {fp8x8_to_bf16(v[0]), fp8x8_to_bf16(v[1])};   // two ahead: a product waits for an operand just written
       __builtin_amdgcn_sched_barrier(0);
@@ -1095,7 +1088,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       each<2 * C::OB>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         acc[i >> 1] = mfma32(a[i & 1], pf[i & 1], acc[i >> 1]);
-        if constexpr (i + VB < 2 * C::OB) v[i % VB] = read(std::integral_constant<int, i + VB>{});
+        if constexpr (i + VB < 2 * C::OB) v[i % VB] = read(i + VB);
         if constexpr (i + 2 < 2 * C::OB) a[i & 1] = fp8x8_to_bf16(v[(i + 2) % VB]);
         beside(ic);
         __builtin_amdgcn_sched_barrier(0);
@@ -1303,8 +1296,8 @@ struct Inst {
 #define QMLA_TR8(DC, K, M, NS, ST, SR) \
   {true, DC, 64 * K, 128 / NS, (const void*)&tree8_kernel<Cfg8<DC, K, M, NS, ST, SR>>, \
    (const void*)&tree_combine_kernel<Cfg8<DC, K, M, NS, ST, SR>>, DC / NS / 32, [](int heads) { return lds_bytes8<Cfg8<DC, K, M, NS, ST, SR>>(heads); }, 16 * SR, !M}
-// the first that fits: FP8 rows as they are where their divisors leave them room (24 heads of any format), staged
-// to bf16 with more
+// the first that fits: FP8 rows as they are where their divisors leave them room (24 heads of one byte), staged to bf16
+// with more
 static const Inst kInst[] = {
     QMLA_TR8(512, 1, false, 1, 6, 39), QMLA_TR8(512, 1, true, 1, 6, 39),
     QMLA_TR8(256, 2, true, 1, 6, 27),  QMLA_TR8(256, 4, true, 1, 6, 35),
