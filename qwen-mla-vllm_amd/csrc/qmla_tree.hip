@@ -735,7 +735,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 // The tiles stay in LDS as the cache holds them, and a wave converts what it multiplies, beside the products. Staged
 // to bf16 (tree_kernel) they cost each workgroup the conversion before its first product of a step, and the LDS
 // twice the bytes: transposed 16-bit reads run at half the LDS rate, 8-bit ones bring 8 tokens of a column in the
-// same time (16 requests of 64 nodes, 2048 .. 8192 tokens: 533 us staged, 323 us so). The rows arrive by LDS-DMA, A tiles ahead, which holds no registers.
+// same time (16 requests of 64 nodes, 2048 .. 8192 tokens: 533 us staged, 337 us so). The rows arrive by LDS-DMA, A tiles ahead, which holds no registers.
 // Scores on the FP8 products (the query as two e4m3 parts) would need no conversion, but those sum with less than fp32:
 // 1.4e-4 off at scores of 5, 5e-6 of the terms, where the bf16 products give 1e-6.
 static_assert(MAXH <= 64);   // divisors: 8 threads a row, 4 heads a thread, twice
